@@ -1,0 +1,336 @@
+// Layer norm over the last axis of [rows, C], forward and backward (with the weights' gradients), for fp32 / fp16 / bf16 rows of any pitch.
+//     y = (x - mean) rstd gamma + beta                       stats[row] = (mean, rstd)
+//     dx = rstd (g - mean(g) - xhat mean(g xhat)) (+ addend), g = dy gamma, xhat = (x - mean) rstd
+//     dgamma = sum_rows dy xhat        dbeta = sum_rows dy
+// Both passes read every tensor once: a row lives in the registers of TPR threads (TPR * NC vectors of 16 bytes), the variance is the mean
+// of squared deviations from the mean (no cancellation between E[x^2] and mean^2).  All sums are fp32.
+//
+// Weight gradients without atomics: a persistent grid, every thread owns the same columns in all its rows and keeps their sums in registers;
+// a workgroup joins its rows' threads through LDS in a fixed order and leaves ONE partial row in the workspace, which a second launch sums.
+// Rows need element alignment only: the 16-byte accesses of this hardware take any address.
+#include "dp_common.h"
+
+namespace {
+
+template <typename X> struct Vec { static constexpr int N = 16 / sizeof(X); };
+
+template <typename X, int N> struct __attribute__((packed, aligned(sizeof(X)))) Pack { X e[N]; };
+
+// N consecutive elements from column col of a row of C; zeros behind its end
+template <typename X, int N>
+__device__ __forceinline__ void ld(const X* row, int col, int C, float* f) {
+    if (col + N <= C) {
+        const Pack<X, N> v = *reinterpret_cast<const Pack<X, N>*>(row + col);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = (float)v.e[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = col + j < C ? (float)row[col + j] : 0.f;
+    }
+}
+template <typename X, int N>
+__device__ __forceinline__ void st(X* row, int col, int C, const float* f) {
+    if (col + N <= C) {
+        Pack<X, N> v;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v.e[j] = (X)f[j];
+        *reinterpret_cast<Pack<X, N>*>(row + col) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (col + j < C) row[col + j] = (X)f[j];
+    }
+}
+
+// sum over the TPR threads of a row; every thread gets it.  red: one slot per wave (TPR > 64 only: two barriers)
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < TPR / 64; ++w) v += red[w];
+    }
+    return v;
+}
+
+template <typename X, typename W, int TPR, int NC>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_kernel(const X* x, long long rows, int C, long long xs, const W* gamma, const W* beta, float eps, X* y,
+                                                                           long long ys, float* stats) {
+    constexpr int N = Vec<X>::N, WGT = TPR > 256 ? TPR : 256, RPB = WGT / TPR;
+    __shared__ float red[WGT / 64];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const float inv_c = 1.f / (float)C;
+    float ga[NC][N], be[NC][N];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int col = (i * TPR + t) * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) { ga[i][j] = 1.f; be[i][j] = 0.f; }
+        if (gamma) ld<W, N>(gamma, col, C, ga[i]);
+        if (beta) ld<W, N>(beta, col, C, be[i]);
+    }
+    for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
+        const long long row = r0 + sub;
+        const bool live = row < rows;
+        const X* xr = x + (live ? row : rows - 1) * xs;
+        float v[NC][N], s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            ld<X, N>(xr, (i * TPR + t) * N, C, v[i]);
+#pragma unroll
+            for (int j = 0; j < N; ++j) s += v[i][j];
+        }
+        const float mean = row_sum<TPR>(s, red) * inv_c;
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int left = C - (i * TPR + t) * N;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                v[i][j] -= mean;
+                q += j < left ? v[i][j] * v[i][j] : 0.f;
+            }
+        }
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) * inv_c + eps);
+        if (!live) continue;
+        X* yr = y + row * ys;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float o[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[j] = fmaf(v[i][j] * rstd, ga[i][j], be[i][j]);
+            st<X, N>(yr, (i * TPR + t) * N, C, o);
+        }
+        if (stats && t == 0) {
+            stats[row * 2] = mean;
+            stats[row * 2 + 1] = rstd;
+        }
+    }
+}
+
+template <typename X, typename W, int TPR, int NC>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(const X* dy, long long dys, const X* x, long long xs, long long rows, int C, const W* gamma,
+                                                                               const float* stats, const X* addend, long long as, X* dx, long long dxs, float* partial) {
+    constexpr int N = Vec<X>::N, WGT = TPR > 256 ? TPR : 256, RPB = WGT / TPR;
+    __shared__ float red[WGT / 64];
+    __shared__ float join[TPR <= 64 ? 2 * TPR * NC * N : 1];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const float inv_c = 1.f / (float)C;
+    float ga[NC][N], dg[NC][N], db[NC][N];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) { ga[i][j] = 1.f; dg[i][j] = 0.f; db[i][j] = 0.f; }
+        if (gamma) ld<W, N>(gamma, (i * TPR + t) * N, C, ga[i]);
+    }
+    for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
+        const long long row = r0 + sub, at = row < rows ? row : rows - 1;
+        const bool live = row < rows;
+        float xh[NC][N], d[NC][N];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            ld<X, N>(x + at * xs, (i * TPR + t) * N, C, xh[i]);
+            ld<X, N>(dy + at * dys, (i * TPR + t) * N, C, d[i]);
+        }
+        const float mean = stats[at * 2], rstd = stats[at * 2 + 1];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                xh[i][j] = (xh[i][j] - mean) * rstd;       // behind the row's end: some value, times dy = 0
+                const float v = live ? d[i][j] : 0.f;
+                dg[i][j] = fmaf(v, xh[i][j], dg[i][j]);
+                db[i][j] += v;
+                d[i][j] *= ga[i][j];
+                s1 += d[i][j];
+                s2 = fmaf(d[i][j], xh[i][j], s2);
+            }
+        s1 = row_sum<TPR>(s1, red) * inv_c;
+        s2 = row_sum<TPR>(s2, red) * inv_c;
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float o[N], a[N];
+            if (addend) ld<X, N>(addend + row * as, (i * TPR + t) * N, C, a);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                o[j] = (d[i][j] - s1 - xh[i][j] * s2) * rstd;
+                if (addend) o[j] += a[j];
+            }
+            st<X, N>(dx + row * dxs, (i * TPR + t) * N, C, o);
+        }
+    }
+    if (!partial) return;
+    float* out = partial + (long long)blockIdx.x * 2 * C;
+    if constexpr (TPR <= 64) {
+        constexpr int P = TPR * NC * N;
+        for (int s = 0; s < RPB; ++s) {
+            if (sub == s) {
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const int at = (i * TPR + t) * N + j;
+                        join[at] = s ? join[at] + dg[i][j] : dg[i][j];
+                        join[P + at] = s ? join[P + at] + db[i][j] : db[i][j];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int cidx = threadIdx.x; cidx < C; cidx += WGT) {
+            out[cidx] = join[cidx];
+            out[C + cidx] = join[P + cidx];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            st<float, N>(out, (i * TPR + t) * N, C, dg[i]);
+            st<float, N>(out + C, (i * TPR + t) * N, C, db[i]);
+        }
+    }
+}
+
+// sums of the partial rows: 64 columns per workgroup, 16 waves share the rows (fixed assignment, fixed order of the join)
+template <typename W>
+__global__ __launch_bounds__(1024) void layer_norm_wsum_kernel(const float* partial, int parts, int C, W* dgamma, W* dbeta) {
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (col < 2 * C)
+        for (int r = wave; r < parts; r += 16) s += partial[(long long)r * 2 * C + col];
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave || col >= 2 * C) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += part[w][lane];
+    W* out = col < C ? dgamma : dbeta;
+    if (out) out[col < C ? col : col - C] = (W)s;
+}
+
+constexpr int MAX_C = 16384;
+constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024;      // persistent grids: 8 / 4 workgroups of 256 threads per CU
+
+struct Plan { int tpr, nc; };
+// a row on as few threads as hold it in 32 floats each: one wave up to 2048 columns (narrow rows share a wave), 256 threads up to 8192, else 1024
+Plan plan(int C, int n) {
+    const int vecs = (C + n - 1) / n;
+    if (vecs <= 16) return {16, 1};
+    if (vecs <= 32) return {32, 1};
+    if (vecs <= 64) return {64, 1};
+    if (vecs <= 128) return {64, 2};
+    if (vecs <= 192) return {64, 3};
+    if (vecs <= 256) return {64, 4};
+    if (n == 4 && vecs <= 512) return {64, 8};
+    if (vecs <= 512) return {256, 2};
+    if (vecs <= 1024) return {256, 4};
+    if (n == 4 && vecs <= 2048) return {256, 8};
+    if (vecs <= 2048) return {1024, 2};
+    return {1024, 4};
+}
+int blocks_of(long long rows, const Plan& p, int most) {
+    const int rpb = p.tpr >= 256 ? 1 : 256 / p.tpr;
+    const long long need = (rows + rpb - 1) / rpb;
+    return (int)(need < most ? need : most);
+}
+
+struct FwdCall {
+    const void* x; long long rows; int C; long long xs; const void *gamma, *beta; float eps; void* y; long long ys; float* stats; hipStream_t s;
+    template <typename X, typename W, int TPR, int NC> void go() const {
+        hipLaunchKernelGGL((layer_norm_kernel<X, W, TPR, NC>), dim3(blocks_of(rows, {TPR, NC}, FWD_BLOCKS)), dim3(TPR > 256 ? TPR : 256), 0, s, (const X*)x, rows, C, xs,
+                           (const W*)gamma, (const W*)beta, eps, (X*)y, ys, stats);
+    }
+};
+struct BwdCall {
+    const void* dy; long long dys; const void* x; long long xs, rows; int C; const void* gamma; const float* stats; const void* addend; long long as; void* dx; long long dxs;
+    float* partial; hipStream_t s;
+    template <typename X, typename W, int TPR, int NC> void go() const {
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<X, W, TPR, NC>), dim3(blocks_of(rows, {TPR, NC}, BWD_BLOCKS)), dim3(TPR > 256 ? TPR : 256), 0, s, (const X*)dy, dys,
+                           (const X*)x, xs, rows, C, (const W*)gamma, stats, (const X*)addend, as, (X*)dx, dxs, partial);
+    }
+};
+template <typename X, typename W, typename Call>
+void dispatch(const Call& c, const Plan& p) {
+    if (p.tpr == 16) c.template go<X, W, 16, 1>();
+    else if (p.tpr == 32) c.template go<X, W, 32, 1>();
+    else if (p.tpr == 64 && p.nc == 1) c.template go<X, W, 64, 1>();
+    else if (p.tpr == 64 && p.nc == 2) c.template go<X, W, 64, 2>();
+    else if (p.tpr == 64 && p.nc == 3) c.template go<X, W, 64, 3>();
+    else if (p.tpr == 64 && p.nc == 4) c.template go<X, W, 64, 4>();
+    else if (p.tpr == 256 && p.nc == 4) c.template go<X, W, 256, 4>();
+    else if constexpr (sizeof(X) == 4) {
+        if (p.tpr == 64) c.template go<X, W, 64, 8>();
+        else if (p.tpr == 256) c.template go<X, W, 256, 8>();
+        else c.template go<X, W, 1024, 4>();
+    } else {
+        if (p.tpr == 256) c.template go<X, W, 256, 2>();
+        else c.template go<X, W, 1024, 2>();
+    }
+}
+template <typename Call>
+void dispatch(const Call& c, int x_dtype, int w_dtype, const Plan& p) {
+    if (x_dtype == 0) dispatch<float, float>(c, p);
+    else if (x_dtype == 1 && w_dtype == 0) dispatch<_Float16, float>(c, p);
+    else if (x_dtype == 1) dispatch<_Float16, _Float16>(c, p);
+    else if (w_dtype == 0) dispatch<__bf16, float>(c, p);
+    else dispatch<__bf16, __bf16>(c, p);
+}
+
+int check(const char* fn, int x_dtype, int w_dtype, long long rows, int C) {
+    DP_REQUIRE(x_dtype >= 0 && x_dtype <= 2, "%s: dtype %d (0 = fp32, 1 = fp16, 2 = bf16)", fn, x_dtype);
+    DP_REQUIRE(w_dtype == 0 || w_dtype == x_dtype, "%s: the weights are fp32 or of the rows' type (got dtype %d)", fn, w_dtype);
+    DP_REQUIRE(rows > 0 && C > 0 && C <= MAX_C, "%s: rows of 1 to %d columns, at least one (got %lld x %d)", fn, MAX_C, rows, C);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int dp_layer_norm(const void* x, int x_dtype, long long rows, int C, long long x_stride, const void* gamma, const void* beta, int w_dtype, float eps, void* y,
+                             long long y_stride, float* stats, void* stream) {
+    const char* fn = "dp_layer_norm";
+    if (int rc = check(fn, x_dtype, w_dtype, rows, C)) return rc;
+    DP_REQUIRE(x && y, "%s: tensor missing", fn);
+    DP_REQUIRE(eps >= 0.f && eps - eps == 0.f, "%s: eps must be finite and not negative", fn);
+    DP_REQUIRE(x_stride >= 0 && (y_stride >= C || rows == 1), "%s: row pitch (x %lld, y %lld; y's rows must not overlap)", fn, x_stride, y_stride);
+    const FwdCall c{x, rows, C, x_stride, gamma, beta, eps, y, y_stride, stats, (hipStream_t)stream};
+    dispatch(c, x_dtype, w_dtype, plan(C, x_dtype == 0 ? 4 : 8));
+    DP_LAUNCH_CHECK("layer_norm");
+    return 0;
+}
+
+extern "C" long long dp_layer_norm_bwd_workspace(long long rows, int C, int x_dtype) {
+    if (rows <= 0 || C <= 0 || C > MAX_C) return 0;
+    return (long long)blocks_of(rows, plan(C, x_dtype == 0 ? 4 : 8), BWD_BLOCKS) * 2 * C * 4;
+}
+
+extern "C" int dp_layer_norm_bwd(const void* dy, long long dy_stride, const void* x, long long x_stride, int x_dtype, long long rows, int C, const void* gamma, int w_dtype,
+                                 const float* stats, const void* addend, long long addend_stride, void* dx, long long dx_stride, void* dgamma, void* dbeta, void* work,
+                                 long long work_bytes, void* stream) {
+    const char* fn = "dp_layer_norm_bwd";
+    if (int rc = check(fn, x_dtype, w_dtype, rows, C)) return rc;
+    DP_REQUIRE(dy && x && stats && dx, "%s: tensor missing", fn);
+    DP_REQUIRE(dy_stride >= 0 && x_stride >= 0 && addend_stride >= 0 && (dx_stride >= C || rows == 1), "%s: row pitch (dx's rows must not overlap)", fn);
+    const bool weights = dgamma || dbeta;
+    DP_REQUIRE(!weights || (work && (reinterpret_cast<uintptr_t>(work) & 3) == 0 && work_bytes >= dp_layer_norm_bwd_workspace(rows, C, x_dtype)),
+               "%s: workspace of %lld bytes needed for the weight gradients (got %lld)", fn, dp_layer_norm_bwd_workspace(rows, C, x_dtype), work_bytes);
+    hipStream_t s = (hipStream_t)stream;
+    const Plan p = plan(C, x_dtype == 0 ? 4 : 8);
+    const BwdCall c{dy, dy_stride, x, x_stride, rows, C, gamma, stats, addend, addend_stride, dx, dx_stride, weights ? (float*)work : nullptr, s};
+    dispatch(c, x_dtype, w_dtype, p);
+    DP_LAUNCH_CHECK("layer_norm_bwd");
+    if (weights) {
+        const int parts = blocks_of(rows, p, BWD_BLOCKS);
+        const dim3 grid((2 * C + 63) / 64);
+        if (w_dtype == 0) hipLaunchKernelGGL(layer_norm_wsum_kernel<float>, grid, dim3(1024), 0, s, (const float*)work, parts, C, (float*)dgamma, (float*)dbeta);
+        else if (w_dtype == 1) hipLaunchKernelGGL(layer_norm_wsum_kernel<_Float16>, grid, dim3(1024), 0, s, (const float*)work, parts, C, (_Float16*)dgamma, (_Float16*)dbeta);
+        else hipLaunchKernelGGL(layer_norm_wsum_kernel<__bf16>, grid, dim3(1024), 0, s, (const float*)work, parts, C, (__bf16*)dgamma, (__bf16*)dbeta);
+        DP_LAUNCH_CHECK("layer_norm_wsum");
+    }
+    return 0;
+}

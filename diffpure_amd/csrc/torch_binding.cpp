@@ -531,6 +531,226 @@ Tensor resize_affine_autograd(const Tensor& x, int64_t ho, int64_t wo, double sh
     return ResizeAffineFn::apply(x, ho, wo, shift, scale, in_nhwc, out_nhwc);
 }
 
+// ---- attention that keeps its log-sum-exp; layer norm (forward, backward, weights' gradients) ------------------------------------------------------
+int dtype_code(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda(), "diffpure_hip: ", name, " must be a GPU tensor (there is no CPU kernel)");
+    const auto st = t.scalar_type();
+    TORCH_CHECK(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, "diffpure_hip: ", name, " must be float32, float16 or bfloat16");
+    return st == at::kFloat ? 0 : (st == at::kHalf ? 1 : 2);
+}
+// (batch, token, head) strides of a [B, T, H, D] tensor like `like`; an axis of length 1 has none
+void head_strides(const Tensor& t, const char* name, const Tensor& like, c10::IntArrayRef shape, long long* st) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.dim() == 4 && t.sizes() == shape, "diffpure_hip: ", name,
+                " must be ", like.scalar_type(), " ", shape, " on ", like.device());
+    for (int i = 0; i < 4; ++i) TORCH_CHECK(t.size(i) <= (1 << 30), "diffpure_hip: ", name, " is too long");
+    TORCH_CHECK(t.size(3) <= 1 || t.stride(3) == 1, "diffpure_hip: ", name, ": the channels of a head must be contiguous");
+    for (int i = 0; i < 3; ++i) st[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+const int* lens_ptr(const c10::optional<Tensor>& t, const char* name, const Tensor& q) {
+    if (!t.has_value() || !t->defined()) return nullptr;
+    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == q.size(0) && t->is_contiguous(), "diffpure_hip: ", name,
+                " must be a contiguous int32 tensor [", q.size(0), "] on ", q.device());
+    return t->data_ptr<int>();
+}
+struct AttnDims {
+    int code, b, tq, tk, hq, hkv, d;
+    float scale;
+    AttnDims(const Tensor& q, const Tensor& k, const Tensor& v, c10::optional<double> sc, long long* st) {
+        code = dtype_code(q, "q");
+        TORCH_CHECK(q.dim() == 4 && k.dim() == 4, "diffpure_hip: q and k must be [B, T, H, D]");
+        head_strides(q, "q", q, q.sizes(), st);
+        const std::vector<int64_t> kv = {q.size(0), k.size(1), k.size(2), q.size(3)};
+        head_strides(k, "k", q, kv, st + 3);
+        head_strides(v, "v", q, kv, st + 6);
+        b = (int)q.size(0); tq = (int)q.size(1); hq = (int)q.size(2); d = (int)q.size(3);
+        tk = (int)k.size(1); hkv = (int)k.size(2);
+        scale = (float)(sc.has_value() ? *sc : 1.0 / std::sqrt((double)std::max(d, 1)));
+    }
+};
+std::tuple<Tensor, Tensor> attention_lse(const Tensor& q, const Tensor& k, const Tensor& v, c10::optional<double> scale, bool causal, const c10::optional<Tensor>& q_lens,
+                                         const c10::optional<Tensor>& kv_lens) {
+    long long st[12];
+    const AttnDims n(q, k, v, scale, st);
+    const int *ql = lens_ptr(q_lens, "q_lens", q), *kl = lens_ptr(kv_lens, "kv_lens", q);
+    c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    head_strides(out, "out", q, q.sizes(), st + 9);
+    DP_CALL(dp_attention_lse(q.data_ptr(), k.data_ptr(), v.data_ptr(), st, n.code, n.b, n.tq, n.tk, n.hq, n.hkv, n.d, ql, kl, n.scale, causal, out.data_ptr(),
+                             lse.data_ptr<float>(), cur_stream(q)));
+    return {out, lse};
+}
+std::tuple<Tensor, Tensor, Tensor> attention_lse_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse,
+                                                     c10::optional<double> scale, bool causal, const c10::optional<Tensor>& q_lens,
+                                                     const c10::optional<Tensor>& kv_lens) {
+    long long st[24];
+    const AttnDims n(q, k, v, scale, st);
+    head_strides(out, "out", q, q.sizes(), st + 9);
+    head_strides(dout, "dout", q, q.sizes(), st + 12);
+    TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 3 && lse.size(0) == n.b && lse.size(1) == n.hq &&
+                    lse.size(2) == n.tq, "diffpure_hip: lse must be contiguous float32 [B, Hq, Tq] on ", q.device());
+    const int *ql = lens_ptr(q_lens, "q_lens", q), *kl = lens_ptr(kv_lens, "kv_lens", q);
+    c10::DeviceGuard guard(q.device());
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), q.options()), dv = at::empty(k.sizes(), q.options());
+    head_strides(dq, "dq", q, q.sizes(), st + 15);
+    head_strides(dk, "dk", q, k.sizes(), st + 18);
+    head_strides(dv, "dv", q, k.sizes(), st + 21);
+    const long long bytes = dp_attention_lse_bwd_workspace(n.b, n.tq, n.hq);
+    Tensor work = at::empty({bytes / 4}, q.options().dtype(at::kFloat));
+    DP_CALL(dp_attention_lse_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(), st, n.code, n.b, n.tq, n.tk, n.hq, n.hkv,
+                                 n.d, ql, kl, n.scale, causal, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), bytes, cur_stream(q)));
+    return {dq, dk, dv};
+}
+
+// rows of a [..., C] tensor at one pitch (elements)
+int64_t row_pitch(const Tensor& t, const char* name, const Tensor& like) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.sizes() == like.sizes() && t.dim() >= 1, "diffpure_hip: ", name,
+                " must be ", like.scalar_type(), " ", like.sizes(), " on ", like.device());
+    TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, "diffpure_hip: ", name, ": the last axis must be contiguous");
+    int64_t pitch = -1, below = 1;
+    for (int64_t i = t.dim() - 2; i >= 0; --i) {
+        if (t.size(i) == 1) continue;
+        if (pitch < 0) pitch = t.stride(i);
+        TORCH_CHECK(t.stride(i) == pitch * below, "diffpure_hip: ", name, ": rows must lie at one pitch");
+        below *= t.size(i);
+    }
+    return pitch < 0 ? t.size(-1) : pitch;
+}
+const void* ln_weight(const c10::optional<Tensor>& w, const char* name, const Tensor& x) {
+    if (!w.has_value() || !w->defined()) return nullptr;
+    TORCH_CHECK(w->device() == x.device() && w->dim() == 1 && w->size(0) == x.size(-1) && w->is_contiguous() && (w->scalar_type() == at::kFloat || w->scalar_type() == x.scalar_type()),
+                "diffpure_hip: ", name, " must be a contiguous tensor [", x.size(-1), "] on ", x.device(), ", float32 or of x's type");
+    return w->data_ptr();
+}
+std::tuple<Tensor, Tensor> layer_norm(const Tensor& x, const c10::optional<Tensor>& gamma, const c10::optional<Tensor>& beta, double eps) {
+    const int code = dtype_code(x, "x");
+    const int64_t pitch = row_pitch(x, "x", x);
+    const void *ga = ln_weight(gamma, "gamma", x), *be = ln_weight(beta, "beta", x);
+    TORCH_CHECK(!ga || !be || gamma->scalar_type() == beta->scalar_type(), "diffpure_hip: gamma and beta must have one type");
+    TORCH_CHECK(x.size(-1) <= (1 << 30), "diffpure_hip: x is too wide");
+    const int64_t c = x.size(-1), rows = c ? x.numel() / c : 0;
+    c10::DeviceGuard guard(x.device());
+    Tensor y = at::empty(x.sizes(), x.options()), stats = at::empty({rows, 2}, x.options().dtype(at::kFloat));
+    DP_CALL(dp_layer_norm(x.data_ptr(), code, rows, (int)c, pitch, ga, be, ga ? dtype_code(*gamma, "gamma") : (be ? dtype_code(*beta, "beta") : 0), (float)eps, y.data_ptr(), c,
+                          stats.data_ptr<float>(), cur_stream(x)));
+    return {y, stats};
+}
+std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x, const c10::optional<Tensor>& gamma, const Tensor& stats,
+                                                  const c10::optional<Tensor>& addend, bool weights) {
+    const int code = dtype_code(x, "x");
+    const int64_t pitch = row_pitch(x, "x", x), dpitch = row_pitch(dy, "dy", x);
+    const bool add = addend.has_value() && addend->defined();
+    const int64_t apitch = add ? row_pitch(*addend, "addend", x) : 0;
+    const void* ga = ln_weight(gamma, "gamma", x);
+    TORCH_CHECK(x.size(-1) <= (1 << 30), "diffpure_hip: x is too wide");
+    const int64_t c = x.size(-1), rows = c ? x.numel() / c : 0;
+    TORCH_CHECK(stats.device() == x.device() && stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.dim() == 2 && stats.size(0) == rows && stats.size(1) == 2,
+                "diffpure_hip: stats must be contiguous float32 [rows, 2] on ", x.device());
+    c10::DeviceGuard guard(x.device());
+    Tensor dx = at::empty(x.sizes(), x.options()), dgamma, dbeta, work;
+    const int wcode = ga ? dtype_code(*gamma, "gamma") : 0;
+    long long bytes = 0;
+    if (weights) {
+        const auto wopt = x.options().dtype(ga ? gamma->scalar_type() : at::kFloat);
+        dgamma = at::empty({c}, wopt);
+        dbeta = at::empty({c}, wopt);
+        bytes = dp_layer_norm_bwd_workspace(rows, (int)c, code);
+        work = at::empty({bytes / 4}, x.options().dtype(at::kFloat));
+    }
+    DP_CALL(dp_layer_norm_bwd(dy.data_ptr(), dpitch, x.data_ptr(), pitch, code, rows, (int)c, ga, wcode, stats.data_ptr<float>(), add ? addend->data_ptr() : nullptr, apitch,
+                              dx.data_ptr(), c, weights ? dgamma.data_ptr() : nullptr, weights ? dbeta.data_ptr() : nullptr, weights ? work.data_ptr() : nullptr, bytes,
+                              cur_stream(x)));
+    return {dx, dgamma, dbeta};
+}
+
+// a cotangent as the kernels read it: channels contiguous, every pitch a multiple of 16 bytes (an expanded one, as sum() leaves it, is laid out)
+Tensor readable(const Tensor& g) {
+    bool ok = g.size(-1) <= 1 || g.stride(-1) == 1;
+    for (int64_t i = 0; i + 1 < g.dim(); ++i) ok = ok && (g.size(i) <= 1 || g.stride(i) * (int64_t)g.element_size() % 16 == 0);
+    ok = ok && reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
+    return ok ? g : g.clone(at::MemoryFormat::Contiguous);
+}
+bool any_grad(std::initializer_list<const Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : ts)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+void no_second(const char* name) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "diffpure_hip: ", name, " has no second derivative (create_graph=True)");
+}
+Tensor or_undefined(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+
+struct AttentionLseFn : public torch::autograd::Function<AttentionLseFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, c10::optional<double> scale, bool causal,
+                                 const c10::optional<Tensor>& q_lens, const c10::optional<Tensor>& kv_lens) {
+        at::AutoDispatchBelowADInplaceOrView g;
+        auto [out, lse] = attention_lse(q, k, v, scale, causal, q_lens, kv_lens);
+        ctx->save_for_backward({q, k, v, out, lse, or_undefined(q_lens), or_undefined(kv_lens)});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["causal"] = causal;
+        ctx->mark_non_differentiable({lse});
+        return {out, lse};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_second("attention_lse");
+        variable_list none(7);
+        if (!grads[0].defined()) return none;
+        const auto s = ctx->get_saved_variables();
+        auto [dq, dk, dv] = attention_lse_bwd(readable(grads[0]), s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toOptional<double>(),
+                                              ctx->saved_data["causal"].toBool(), s[5], s[6]);
+        none[0] = dq;
+        none[1] = dk;
+        none[2] = dv;
+        return none;
+    }
+};
+std::tuple<Tensor, Tensor> attention_lse_autograd(const Tensor& q, const Tensor& k, const Tensor& v, c10::optional<double> scale, bool causal,
+                                                  const c10::optional<Tensor>& q_lens, const c10::optional<Tensor>& kv_lens) {
+    if (!any_grad({&q, &k, &v})) {
+        at::AutoDispatchBelowADInplaceOrView g;
+        return attention_lse(q, k, v, scale, causal, q_lens, kv_lens);
+    }
+    auto r = AttentionLseFn::apply(q, k, v, scale, causal, q_lens, kv_lens);
+    return {r[0], r[1]};
+}
+
+struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& gamma_, const c10::optional<Tensor>& beta_, double eps) {
+        at::AutoDispatchBelowADInplaceOrView g;
+        const Tensor gamma = or_undefined(gamma_), beta = or_undefined(beta_);
+        auto [y, stats] = layer_norm(x, gamma_, beta_, eps);
+        ctx->save_for_backward({x, gamma, stats});
+        const bool wg = gamma.defined() && gamma.requires_grad(), wb = beta.defined() && beta.requires_grad();
+        ctx->saved_data["weights"] = wg || wb;
+        ctx->saved_data["beta_type"] = (int64_t)(beta.defined() ? beta.scalar_type() : at::kFloat);
+        ctx->saved_data["has_beta"] = beta.defined();
+        ctx->mark_non_differentiable({stats});
+        return {y, stats};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_second("layer_norm");
+        variable_list none(4);
+        if (!grads[0].defined()) return none;
+        const auto s = ctx->get_saved_variables();
+        Tensor dy = grads[0];
+        if (dy.dim() > 1 || dy.stride(-1) != 1) dy = dy.contiguous();
+        auto [dx, dgamma, dbeta] = layer_norm_bwd(dy, s[0], s[1], s[2], c10::nullopt, ctx->saved_data["weights"].toBool());
+        none[0] = dx;
+        if (s[1].defined()) none[1] = dgamma;
+        if (ctx->saved_data["has_beta"].toBool() && dbeta.defined()) none[2] = dbeta.to((at::ScalarType)ctx->saved_data["beta_type"].toInt());
+        return none;
+    }
+};
+std::tuple<Tensor, Tensor> layer_norm_autograd(const Tensor& x, const c10::optional<Tensor>& gamma, const c10::optional<Tensor>& beta, double eps) {
+    const Tensor ga = or_undefined(gamma), be = or_undefined(beta);
+    if (!any_grad({&x, &ga, &be})) {
+        at::AutoDispatchBelowADInplaceOrView g;
+        return layer_norm(x, gamma, beta, eps);
+    }
+    auto r = LayerNormFn::apply(x, gamma, beta, eps);
+    return {r[0], r[1]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(diffpure_hip, m) {
@@ -559,6 +779,12 @@ TORCH_LIBRARY(diffpure_hip, m) {
     m.def("attention_bwd(Tensor qkv, Tensor dout, int n_heads, bool legacy_layout) -> Tensor");
     m.def("resize_affine_bwd(Tensor dy, int hi, int wi, float scale, bool in_nhwc, bool out_nhwc) -> Tensor");
     m.def("conv2d_nhwc_dgrad(Tensor dy, Tensor wp, int c_in, int ksize) -> Tensor");
+    // attention from / to its log-sum-exp and layer norm, with every gradient
+    m.def("attention_lse(Tensor q, Tensor k, Tensor v, float? scale=None, bool causal=False, Tensor? q_lens=None, Tensor? kv_lens=None) -> (Tensor, Tensor)");
+    m.def("attention_lse_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, float? scale=None, bool causal=False, Tensor? q_lens=None, "
+          "Tensor? kv_lens=None) -> (Tensor, Tensor, Tensor)");
+    m.def("layer_norm(Tensor x, Tensor? gamma=None, Tensor? beta=None, float eps=1e-5) -> (Tensor, Tensor)");
+    m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor? gamma, Tensor stats, Tensor? addend=None, bool weights=True) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(diffpure_hip, CUDA, m) {      // CUDA dispatch key = HIP devices on a ROCm build; no CPU implementation
@@ -581,6 +807,10 @@ TORCH_LIBRARY_IMPL(diffpure_hip, CUDA, m) {      // CUDA dispatch key = HIP devi
     m.impl("attention_bwd", attention_bwd);
     m.impl("resize_affine_bwd", resize_affine_bwd);
     m.impl("conv2d_nhwc_dgrad", conv2d_nhwc_dgrad);
+    m.impl("attention_lse", attention_lse);
+    m.impl("attention_lse_bwd", attention_lse_bwd);
+    m.impl("layer_norm", layer_norm);
+    m.impl("layer_norm_bwd", layer_norm_bwd);
 }
 
 // torch.autograd through the operators: conv2d_nhwc, group_norm_silu (fp32 output form), attention and resize_affine carry dL/dx
@@ -591,4 +821,6 @@ TORCH_LIBRARY_IMPL(diffpure_hip, Autograd, m) {
     m.impl("group_norm_silu", group_norm_silu_autograd);
     m.impl("attention", attention_autograd);
     m.impl("resize_affine", resize_affine_autograd);
+    m.impl("attention_lse", attention_lse_autograd);      // dq, dk, dv
+    m.impl("layer_norm", layer_norm_autograd);            // dx and the weights' gradients
 }

@@ -1060,6 +1060,160 @@ def attention_bwd(qkv, probs, dout, n_heads, layout, h16=False):
     return dqkv
 
 
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _heads(t, name, like=None, shape=None):
+    """a [B, T, H, D] GPU tensor of a kernel type with contiguous channels -> its (batch, token, head) strides in elements"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 4 or t.dtype not in _DTYPES:
+        raise _lib.DiffpureHipError(f"{name}: expected a [B, T, H, D] fp32 / fp16 / bf16 GPU tensor")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise _lib.DiffpureHipError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise _lib.DiffpureHipError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
+    if max(t.shape) > 1 << 30:
+        raise _lib.DiffpureHipError(f"{name}: {tuple(t.shape)} is too long an axis")
+    if t.stride(3) != 1 and t.shape[3] > 1:
+        raise _lib.DiffpureHipError(f"{name}: the channels of a head must be contiguous (strides {t.stride()})")
+    # an axis of length 1 has no stride to speak of
+    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
+
+
+def _lens(t, name, q):
+    if t is not None and (not isinstance(t, torch.Tensor) or t.device != q.device or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != q.shape[0] or not t.is_contiguous()):
+        raise _lib.DiffpureHipError(f"{name}: expected a contiguous int32 tensor [{q.shape[0]}] on {q.device}")
+    return t
+
+
+def _attn_lse_args(fn, q, k, v, scale, q_lens, kv_lens):
+    st = _heads(q, f"{fn}.q")
+    b, tq, hq, d = q.shape
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise _lib.DiffpureHipError(f"{fn}.k: expected a [B, T, H, D] tensor")
+    tk, hkv = k.shape[1], k.shape[2]
+    st += _heads(k, f"{fn}.k", q, (b, tk, hkv, d)) + _heads(v, f"{fn}.v", q, (b, tk, hkv, d))
+    _lens(q_lens, f"{fn}.q_lens", q)
+    _lens(kv_lens, f"{fn}.kv_lens", q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(max(d, 1))
+    return st, (_DTYPES[q.dtype], b, tq, tk, hq, hkv, d, _ptr(q_lens), _ptr(kv_lens), float(scale))
+
+
+def attention_lse(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
+    """softmax(scale q k^T + mask) v and the log-sum-exp of its rows: q [B, Tq, Hq, D], k, v [B, Tk, Hkv, D] -> out [B, Tq, Hq, D] (contiguous),
+    lse [B, Hq, Tq] fp32.  fp32 / fp16 / bf16, any strides that are multiples of 16 bytes (views of one qkv tensor in either head order), any token
+    counts, D a multiple of 8 up to 256, Hq a multiple of Hkv (query heads h * Hq / Hkv ... share key head h); scale None = 1 / sqrt(D).
+    q_lens / kv_lens: int32 [B], valid tokens per sample; causal: the last valid row sees every valid key, each row before it one fewer.
+    Rows that see nothing give 0 and -inf.  The statistics are what attention_lse_bwd recomputes the probabilities from (csrc/attention_lse.hip)."""
+    st, args = _attn_lse_args("attention_lse", q, k, v, scale, q_lens, kv_lens)
+    b, tq, hq, d = q.shape
+    with torch.cuda.device(q.device):
+        out = torch.empty((b, tq, hq, d), device=q.device, dtype=q.dtype)
+        lse = torch.empty((b, hq, tq), device=q.device, dtype=torch.float32)
+        st = (ctypes.c_longlong * 12)(*st, *out.stride()[:3])
+        _lib.call("dp_attention_lse", _ptr(q), _ptr(k), _ptr(v), ctypes.addressof(st), *args, int(bool(causal)), _ptr(out), _ptr(lse), _stream())
+    return out, lse
+
+
+def attention_lse_bwd(dout, q, k, v, out, lse, scale=None, causal=False, q_lens=None, kv_lens=None, grads=None):
+    """Gradients (dq, dk, dv) of attention_lse's `out` for the cotangent dout, given its results and the arguments of the forward call.  No [Tq, Tk] tensor
+    and no atomics; a key head's gradient is the sum over the query heads that share it.  grads=(dq, dk, dv): written into these tensors (of
+    q's type; views of one dqkv tensor, say) instead of new contiguous ones."""
+    st, args = _attn_lse_args("attention_lse_bwd", q, k, v, scale, q_lens, kv_lens)
+    b, tq, hq, d = q.shape
+    st += _heads(out, "attention_lse_bwd.out", q, q.shape) + _heads(dout, "attention_lse_bwd.dout", q, q.shape)
+    if not isinstance(lse, torch.Tensor) or lse.device != q.device or lse.dtype != torch.float32 or tuple(lse.shape) != (b, hq, tq) or not lse.is_contiguous():
+        raise _lib.DiffpureHipError(f"attention_lse_bwd.lse: expected contiguous float32 {(b, hq, tq)} on {q.device}")
+    with torch.cuda.device(q.device):
+        if grads is None:
+            grads = tuple(torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+        dq, dk, dv = grads
+        for t, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
+            st += _heads(t, f"attention_lse_bwd.{name}", q, like.shape)
+        st = (ctypes.c_longlong * 24)(*st)
+        nbytes = _lib.load().dp_attention_lse_bwd_workspace(b, tq, hq)
+        work = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32)
+        _lib.call("dp_attention_lse_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), ctypes.addressof(st), *args, int(bool(causal)),
+                  _ptr(dq), _ptr(dk), _ptr(dv), _ptr(work), nbytes, _stream())
+    return dq, dk, dv
+
+
+# ---------------------------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------------------------
+def _rows(t, name, like=None):
+    """[..., C] GPU tensor whose rows lie at one pitch -> (rows, C, pitch in elements)"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() < 1 or t.dtype not in _DTYPES:
+        raise _lib.DiffpureHipError(f"{name}: expected a [..., C] fp32 / fp16 / bf16 GPU tensor")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise _lib.DiffpureHipError(f"{name}: expected {like.dtype} {tuple(like.shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    c = t.shape[-1]
+    rows = t.numel() // c if c else 0
+    pitch, below = None, 1
+    for i in range(t.dim() - 2, -1, -1):
+        if t.shape[i] == 1:
+            continue
+        if pitch is None:
+            pitch = t.stride(i)
+        if t.stride(i) != pitch * below:
+            raise _lib.DiffpureHipError(f"{name}: rows must lie at one pitch (shape {tuple(t.shape)}, strides {t.stride()})")
+        below *= t.shape[i]
+    if c > 1 and t.stride(-1) != 1:
+        raise _lib.DiffpureHipError(f"{name}: the last axis must be contiguous (strides {t.stride()})")
+    return rows, c, c if pitch is None else pitch
+
+
+def _ln_weight(w, name, x):
+    if w is None:
+        return None
+    if not isinstance(w, torch.Tensor) or w.device != x.device or tuple(w.shape) != (x.shape[-1],) or not w.is_contiguous() or w.dtype not in (torch.float32, x.dtype):
+        raise _lib.DiffpureHipError(f"{name}: expected a contiguous tensor [{x.shape[-1]}] on {x.device}, float32 or {x.dtype}")
+    return w
+
+
+def _ln_wtype(fn, gamma, beta):
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise _lib.DiffpureHipError(f"{fn}: gamma and beta must have one type")
+    w = gamma if gamma is not None else beta
+    return 0 if w is None else _DTYPES[w.dtype]
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-5):
+    """(x - mean) * rstd * gamma + beta over the last axis (1 .. 16384 wide) of a [..., C] tensor, fp32 / fp16 / bf16, rows at one pitch ->
+    (y contiguous, stats [rows, 2] fp32 = (mean, rstd)).  gamma / beta: fp32 or x's type, or None."""
+    rows, c, pitch = _rows(x, "layer_norm.x")
+    _ln_weight(gamma, "layer_norm.gamma", x)
+    _ln_weight(beta, "layer_norm.beta", x)
+    with torch.cuda.device(x.device):
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32)
+        _lib.call("dp_layer_norm", _ptr(x), _DTYPES[x.dtype], rows, c, pitch, _ptr(gamma), _ptr(beta), _ln_wtype("layer_norm", gamma, beta), float(eps), _ptr(y), c,
+                  _ptr(stats), _stream())
+    return y, stats
+
+
+def layer_norm_bwd(dy, x, gamma, stats, addend=None, weights=True):
+    """Gradient of layer_norm -> (dx contiguous, dgamma, dbeta); the weights' gradients in gamma's type (fp32 without a gamma), None with weights=False.
+    addend: a tensor like x added to dx (the gradient of the residual branch around the norm)."""
+    rows, c, pitch = _rows(x, "layer_norm_bwd.x")
+    _, _, dpitch = _rows(dy, "layer_norm_bwd.dy", x)
+    apitch = _rows(addend, "layer_norm_bwd.addend", x)[2] if addend is not None else 0
+    _ln_weight(gamma, "layer_norm_bwd.gamma", x)
+    if not isinstance(stats, torch.Tensor) or stats.device != x.device or stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 2) or not stats.is_contiguous():
+        raise _lib.DiffpureHipError(f"layer_norm_bwd.stats: expected contiguous float32 {(rows, 2)} on {x.device}")
+    with torch.cuda.device(x.device):
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        dgamma = dbeta = work = None
+        nbytes = 0
+        if weights:
+            dgamma, dbeta = (torch.empty((c,), device=x.device, dtype=torch.float32 if gamma is None else gamma.dtype) for _ in range(2))
+            nbytes = _lib.load().dp_layer_norm_bwd_workspace(rows, c, _DTYPES[x.dtype])
+            work = torch.empty((nbytes // 4,), device=x.device, dtype=torch.float32)
+        _lib.call("dp_layer_norm_bwd", _ptr(dy), dpitch, _ptr(x), pitch, _DTYPES[x.dtype], rows, c, _ptr(gamma), _ln_wtype("layer_norm_bwd", gamma, None), _ptr(stats),
+                  _ptr(addend), apitch, _ptr(dx), c, _ptr(dgamma), _ptr(dbeta), _ptr(work), nbytes, _stream())
+    return dx, dgamma, dbeta
+
+
 # ---------------------------------------------------------------------------------------------
 # small pieces
 # ---------------------------------------------------------------------------------------------

@@ -31,6 +31,11 @@ ABI 6 / 7 (rounds 4-5) - the fp16 residual stream and the backward entry points:
     group_norm_stats, group_norm_silu_bwd, attention_bwd, resize_affine_bwd, conv2d_nhwc_dgrad      backward entry points (dL/dx)
 ABI 8 (round 6):
     conv2d_stem                          the 3 -> N stem convolution as a write-bound kernel (22-bit operands, three fp16 MFMA passes)
+A transformer block's operators (fp32 / fp16 / bf16; a classifier behind the purifier and the attacks' and fine-tuning's gradients through it):
+    attention_lse, attention_lse_bwd     softmax(scale q k^T + mask) v on [B, T, H, D] views with the rows' log-sum-exp; dq, dk, dv with the
+                                         probabilities recomputed from it.  Any token counts, shared key heads, per-sample lengths, causal
+    layer_norm, layer_norm_bwd           (y, stats); (dx [+ the residual branch's gradient], dgamma, dbeta)
+    Both forwards carry gradients for every floating input (weights included); lse and stats are not differentiable, second derivatives raise.
 torch.autograd: conv2d_nhwc, group_norm_silu (fp32 output form), attention and resize_affine are registered for the Autograd key with
 dL/dx formulas built from those entry points (weights are constants on this path): `y.backward()` / `torch.autograd.grad` work through them.
 """
@@ -44,7 +49,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "lib
 OPERATORS = ("conv2d_nhwc", "conv2d_nhwc_stats", "conv2d_h2", "conv2d_h2_stats", "group_norm_stats_from_cols", "group_norm_silu",
              "attention", "em_step", "resize_affine",
              "conv2d_h2_ex", "gn_apply_h16", "attention_fused", "round_weights", "group_norm_stats", "group_norm_silu_bwd", "attention_bwd",
-             "resize_affine_bwd", "conv2d_nhwc_dgrad", "conv2d_stem")
+             "resize_affine_bwd", "conv2d_nhwc_dgrad", "conv2d_stem", "attention_lse", "attention_lse_bwd", "layer_norm", "layer_norm_bwd")
 
 if not os.path.exists(LIB_PATH):
     raise _lib.DiffpureHipError(f"{LIB_PATH} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`")

@@ -404,6 +404,47 @@ int dp_resize_affine(const float* x, int B, int C, int Hi, int Wi, int in_nhwc, 
 int dp_resize_affine_bwd(const float* dy, int B, int C, int Ho, int Wo, int out_nhwc, float scale, float* dx, int Hi,
                          int Wi, int in_nhwc, void* stream);
 
+/* ---- attention that keeps its log-sum-exp, and its backward pass ---------------------------------------------------
+ * out = softmax(scale q k^T + mask) v and lse[b][h][i] = log sum_j exp(scale q_i k_j) over the keys that row i sees; the backward pass recomputes the
+ * probabilities from lse tile by tile: nothing of size Tq x Tk is ever stored (dp_softmax_rows / dp_softmax_bwd_rows work on the stored scores).
+ *   q, out, dout, dq: [B][Tq][Hq][D]     k, v, dk, dv: [B][Tk][Hkv][D]     any strides; channels contiguous.  Hq a multiple of Hkv: query head h
+ *     reads key head h / (Hq / Hkv), whose gradient is the sum over the heads that share it.  D a multiple of 8 up to 256.
+ *   dtype 0 = fp32 (fp32 matrix products throughout), 1 = fp16, 2 = bf16 (16-bit operands, fp32 scores, sums and gradients in flight; the
+ *     probabilities and dS are rounded to the type as operands of their products): one type for all of these tensors; lse is fp32 [B][Hq][Tq].
+ *   strides: HOST array, 3 per tensor (batch, token, head) in elements, multiples of 16 bytes - forward: q, k, v, out (12 values); backward: q, k, v,
+ *     out, dout, dq, dk, dv (24 values).  Base pointers 16-byte aligned.  A read tensor may have stride 0 (an expanded one).  So q, k, v and their
+ *     gradients may be views of one [B][T][3C] tensor in either head order (dp_attention_fused's layouts).
+ *   q_lens, kv_lens: device int32 [B] or NULL - the valid tokens of each sample (values outside 0 .. T are clamped).  Rows and keys behind them may
+ *     hold anything (NaN too): their out and gradients are written as 0, their lse as -inf.
+ *   causal != 0: row i of a sample sees keys 0 .. i + (keys - rows) of it (the last row sees every key).  Inside the lengths values must be finite for the mask to
+ *     hide them.  A row that sees no key has out 0, lse -inf, and contributes no gradient.
+ *   scale: finite, not 0.
+ *   work of the backward pass: dp_attention_lse_bwd_workspace(B, Tq, Hq) bytes, 16-byte aligned, free again when the call's work on `stream` is
+ *     done.  The outputs may not overlap any input.  Results do not depend on the order in which workgroups run (no atomics).
+ * The reference has no counterpart that keeps the statistics (QKVAttentionLegacy.forward, guided_diffusion/unet.py:345-362, materialises the weights and
+ * autograd keeps or checkpoints them). */
+int dp_attention_lse(const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
+                     const int* q_lens, const int* kv_lens, float scale, int causal, void* out, float* lse, void* stream);
+long long dp_attention_lse_bwd_workspace(int B, int Tq, int Hq);
+int dp_attention_lse_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides, int dtype,
+                         int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, void* dq, void* dk,
+                         void* dv, void* work, long long work_bytes, void* stream);
+
+/* ---- layer norm over the last axis, and its backward pass with the weights' gradients ---------------------------------
+ *   y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(var + eps) (biased variance); stats[row] = (mean, rstd) fp32, or NULL.
+ *   dx = rstd (g - mean(g) - xhat mean(g xhat)) [+ addend], g = dy gamma; dgamma = sum over rows of dy xhat, dbeta = sum over rows of dy.
+ *   x, y, dy, addend, dx: `rows` rows of C (1 .. 16384) contiguous elements, one type (x_dtype 0 = fp32, 1 = fp16, 2 = bf16), row pitches in
+ *     elements (a read tensor may have pitch 0); any element alignment.  gamma, beta (each may be NULL: 1 and 0), dgamma, dbeta (each may be NULL:
+ *     not formed): w_dtype 0 = fp32 or x_dtype.  Sums are fp32; the order of the sums is fixed by (rows, C, type).
+ *   work: dp_layer_norm_bwd_workspace(rows, C, x_dtype) bytes where dgamma or dbeta is formed, 4-byte aligned.
+ * No reference counterpart in the purifier (its norms are GroupNorms); transformer classifiers behind it (utils.py:143-253's zoo) are built on it. */
+int dp_layer_norm(const void* x, int x_dtype, long long rows, int C, long long x_stride, const void* gamma, const void* beta, int w_dtype, float eps, void* y,
+                  long long y_stride, float* stats, void* stream);
+long long dp_layer_norm_bwd_workspace(long long rows, int C, int x_dtype);
+int dp_layer_norm_bwd(const void* dy, long long dy_stride, const void* x, long long x_stride, int x_dtype, long long rows, int C, const void* gamma, int w_dtype,
+                      const float* stats, const void* addend, long long addend_stride, void* dx, long long dx_stride, void* dgamma, void* dbeta, void* work,
+                      long long work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
