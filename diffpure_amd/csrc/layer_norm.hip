@@ -8,39 +8,34 @@
 // Weight gradients without atomics: a persistent grid, every thread owns the same columns in all its rows and keeps their sums in registers;
 // a workgroup joins its rows' threads through LDS in a fixed order and leaves ONE partial row in the workspace, which a second launch sums.
 // Rows need element alignment only: the 16-byte accesses of this hardware take any address.
+//
+// Bound by memory: each row's loads are issued one row ahead of their use.  MI355X (a 1 GiB copy runs at 5.2 TB/s): forward 50 432 x 768 bf16
+// 29.3 us = 5.3 TB/s; backward with weight gradients and addend 60.4 us = 5.1 TB/s; backward 5 003 x 1001 fp32 16.3 us = 3.7 TB/s (two launches);
+// forward 64 x 768 6 us, the time of a launch.  The variant of plan() goes by the row's width only.
 #include "dp_common.h"
 
 namespace {
 
-template <typename X> struct Vec { static constexpr int N = 16 / sizeof(X); };
-
 template <typename X, int N> struct __attribute__((packed, aligned(sizeof(X)))) Pack { X e[N]; };
+template <typename X, int N> __device__ __forceinline__ Pack<X, N> ld(const X* p) { return *reinterpret_cast<const Pack<X, N>*>(p); }
+template <typename X, int N> __device__ __forceinline__ void st(X* p, const float* f) {
+    Pack<X, N> v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v.e[j] = (X)f[j];
+    *reinterpret_cast<Pack<X, N>*>(p) = v;
+}
 
-// N consecutive elements from column col of a row of C; zeros behind its end
-template <typename X, int N>
-__device__ __forceinline__ void ld(const X* row, int col, int C, float* f) {
-    if (col + N <= C) {
-        const Pack<X, N> v = *reinterpret_cast<const Pack<X, N>*>(row + col);
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = (float)v.e[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = col + j < C ? (float)row[col + j] : 0.f;
+// Columns of a thread's vector: the vector that would reach behind the row's end is moved back to end with it (C >= N), so every access is a whole
+// vector and nothing branches.  Its first `skip` columns then belong to the vector before it: both threads compute and store the same values
+// there; only the sums over the row leave them out.  A thread without columns repeats the last vector and skips all of it.
+template <int N> struct Cols {
+    int at, skip;
+    __device__ __forceinline__ Cols(int vec, int C) {
+        const int want = vec * N;
+        at = want + N <= C ? want : C - N;
+        skip = want - at;
     }
-}
-template <typename X, int N>
-__device__ __forceinline__ void st(X* row, int col, int C, const float* f) {
-    if (col + N <= C) {
-        Pack<X, N> v;
-#pragma unroll
-        for (int j = 0; j < N; ++j) v.e[j] = (X)f[j];
-        *reinterpret_cast<Pack<X, N>*>(row + col) = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (col + j < C) row[col + j] = (X)f[j];
-    }
-}
+};
 
 // sum over the TPR threads of a row; every thread gets it.  red: one slot per wave (TPR > 64 only: two barriers)
 template <int TPR>
@@ -58,53 +53,68 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return v;
 }
 
-template <typename X, typename W, int TPR, int NC>
+template <typename X, typename W, int N, int TPR, int NC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_kernel(const X* x, long long rows, int C, long long xs, const W* gamma, const W* beta, float eps, X* y,
                                                                            long long ys, float* stats) {
-    constexpr int N = Vec<X>::N, WGT = TPR > 256 ? TPR : 256, RPB = WGT / TPR;
+    constexpr int WGT = TPR > 256 ? TPR : 256, RPB = WGT / TPR;
     __shared__ float red[WGT / 64];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const float inv_c = 1.f / (float)C;
     float ga[NC][N], be[NC][N];
+    int at[NC], skip[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int col = (i * TPR + t) * N;
+        const Cols<N> c(i * TPR + t, C);
+        at[i] = c.at;
+        skip[i] = c.skip;
 #pragma unroll
         for (int j = 0; j < N; ++j) { ga[i][j] = 1.f; be[i][j] = 0.f; }
-        if (gamma) ld<W, N>(gamma, col, C, ga[i]);
-        if (beta) ld<W, N>(beta, col, C, be[i]);
+        if (gamma) {
+            const Pack<W, N> w = ld<W, N>(gamma + c.at);
+#pragma unroll
+            for (int j = 0; j < N; ++j) ga[i][j] = (float)w.e[j];
+        }
+        if (beta) {
+            const Pack<W, N> w = ld<W, N>(beta + c.at);
+#pragma unroll
+            for (int j = 0; j < N; ++j) be[i][j] = (float)w.e[j];
+        }
     }
-    for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
-        const long long row = r0 + sub;
-        const bool live = row < rows;
-        const X* xr = x + (live ? row : rows - 1) * xs;
+    const long long step = (long long)gridDim.x * RPB;
+    long long row = (long long)blockIdx.x * RPB + sub;
+    Pack<X, N> raw[NC];                                  // a row ahead: the next row's loads are under way while this one is reduced
+#pragma unroll
+    for (int i = 0; i < NC; ++i) raw[i] = ld<X, N>(x + (row < rows ? row : rows - 1) * xs + at[i]);
+    for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += step, row += step) {
         float v[NC][N], s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            ld<X, N>(xr, (i * TPR + t) * N, C, v[i]);
+        for (int i = 0; i < NC; ++i)
 #pragma unroll
-            for (int j = 0; j < N; ++j) s += v[i][j];
-        }
+            for (int j = 0; j < N; ++j) {
+                v[i][j] = (float)raw[i].e[j];
+                s += j >= skip[i] ? v[i][j] : 0.f;
+            }
+        const long long next = row + step < rows ? row + step : rows - 1;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) raw[i] = ld<X, N>(x + next * xs + at[i]);
         const float mean = row_sum<TPR>(s, red) * inv_c;
         float q = 0.f;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int left = C - (i * TPR + t) * N;
+        for (int i = 0; i < NC; ++i)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 v[i][j] -= mean;
-                q += j < left ? v[i][j] * v[i][j] : 0.f;
+                q += j >= skip[i] ? v[i][j] * v[i][j] : 0.f;
             }
-        }
         const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) * inv_c + eps);
-        if (!live) continue;
+        if (row >= rows) continue;
         X* yr = y + row * ys;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             float o[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) o[j] = fmaf(v[i][j] * rstd, ga[i][j], be[i][j]);
-            st<X, N>(yr, (i * TPR + t) * N, C, o);
+            if (skip[i] < N) st<X, N>(yr + at[i], o);
         }
         if (stats && t == 0) {
             stats[row * 2] = mean;
@@ -113,114 +123,163 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_kernel(const
     }
 }
 
-template <typename X, typename W, int TPR, int NC>
+template <typename X, typename W, int N, int TPR, int NC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(const X* dy, long long dys, const X* x, long long xs, long long rows, int C, const W* gamma,
                                                                                const float* stats, const X* addend, long long as, X* dx, long long dxs, float* partial) {
-    constexpr int N = Vec<X>::N, WGT = TPR > 256 ? TPR : 256, RPB = WGT / TPR;
-    __shared__ float red[WGT / 64];
+    constexpr int WGT = TPR > 256 ? TPR : 256, RPB = WGT / TPR;
+    __shared__ float red[2][WGT / 64];
     __shared__ float join[TPR <= 64 ? 2 * TPR * NC * N : 1];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const float inv_c = 1.f / (float)C;
     float ga[NC][N], dg[NC][N], db[NC][N];
+    int at[NC], skip[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
+        const Cols<N> c(i * TPR + t, C);
+        at[i] = c.at;
+        skip[i] = c.skip;
 #pragma unroll
         for (int j = 0; j < N; ++j) { ga[i][j] = 1.f; dg[i][j] = 0.f; db[i][j] = 0.f; }
-        if (gamma) ld<W, N>(gamma, (i * TPR + t) * N, C, ga[i]);
+        if (gamma) {
+            const Pack<W, N> w = ld<W, N>(gamma + c.at);
+#pragma unroll
+            for (int j = 0; j < N; ++j) ga[i][j] = (float)w.e[j];
+        }
     }
-    for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
-        const long long row = r0 + sub, at = row < rows ? row : rows - 1;
-        const bool live = row < rows;
-        float xh[NC][N], d[NC][N];
+    const long long step = (long long)gridDim.x * RPB;
+    long long row = (long long)blockIdx.x * RPB + sub;
+    Pack<X, N> rx[NC], rd[NC], ra[NC];                   // a row ahead
+    float rmean, rrstd;
+    auto fetch = [&](long long r) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            ld<X, N>(x + at * xs, (i * TPR + t) * N, C, xh[i]);
-            ld<X, N>(dy + at * dys, (i * TPR + t) * N, C, d[i]);
+            rx[i] = ld<X, N>(x + r * xs + at[i]);
+            rd[i] = ld<X, N>(dy + r * dys + at[i]);
         }
-        const float mean = stats[at * 2], rstd = stats[at * 2 + 1];
-        float s1 = 0.f, s2 = 0.f;
+        rmean = stats[r * 2];
+        rrstd = stats[r * 2 + 1];
+    };
+    fetch(row < rows ? row : rows - 1);
+    for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += step, row += step) {
+        const bool live = row < rows;
+        const float mean = rmean, rstd = rrstd;
+        float xh[NC][N], d[NC][N], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                xh[i][j] = (xh[i][j] - mean) * rstd;       // behind the row's end: some value, times dy = 0
+                xh[i][j] = (float)rx[i].e[j];
+                d[i][j] = (float)rd[i].e[j];
+            }
+        if (addend) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) ra[i] = ld<X, N>(addend + (live ? row : rows - 1) * as + at[i]);
+        }
+        fetch(row + step < rows ? row + step : rows - 1);
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                xh[i][j] = (xh[i][j] - mean) * rstd;
                 const float v = live ? d[i][j] : 0.f;
                 dg[i][j] = fmaf(v, xh[i][j], dg[i][j]);
                 db[i][j] += v;
                 d[i][j] *= ga[i][j];
-                s1 += d[i][j];
-                s2 = fmaf(d[i][j], xh[i][j], s2);
+                const float g = j >= skip[i] ? d[i][j] : 0.f;
+                s1 += g;
+                s2 = fmaf(g, xh[i][j], s2);
             }
-        s1 = row_sum<TPR>(s1, red) * inv_c;
-        s2 = row_sum<TPR>(s2, red) * inv_c;
+        s1 = row_sum<TPR>(s1, red[0]) * inv_c;
+        s2 = row_sum<TPR>(s2, red[1]) * inv_c;
         if (!live) continue;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            float o[N], a[N];
-            if (addend) ld<X, N>(addend + row * as, (i * TPR + t) * N, C, a);
+            float o[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 o[j] = (d[i][j] - s1 - xh[i][j] * s2) * rstd;
-                if (addend) o[j] += a[j];
+                if (addend) o[j] += (float)ra[i].e[j];
             }
-            st<X, N>(dx + row * dxs, (i * TPR + t) * N, C, o);
+            if (skip[i] < N) st<X, N>(dx + row * dxs + at[i], o);
         }
     }
     if (!partial) return;
     float* out = partial + (long long)blockIdx.x * 2 * C;
     if constexpr (TPR <= 64) {
-        constexpr int P = TPR * NC * N;
+        constexpr int P = TPR * NC * N;                  // by vector, not by column: no two threads of a row share a place
         for (int s = 0; s < RPB; ++s) {
             if (sub == s) {
 #pragma unroll
                 for (int i = 0; i < NC; ++i)
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
-                        const int at = (i * TPR + t) * N + j;
-                        join[at] = s ? join[at] + dg[i][j] : dg[i][j];
-                        join[P + at] = s ? join[P + at] + db[i][j] : db[i][j];
+                        const int k = (i * N + j) * TPR + t;
+                        join[k] = s ? join[k] + dg[i][j] : dg[i][j];
+                        join[P + k] = s ? join[P + k] + db[i][j] : db[i][j];
                     }
             }
             __syncthreads();
         }
-        for (int cidx = threadIdx.x; cidx < C; cidx += WGT) {
-            out[cidx] = join[cidx];
-            out[C + cidx] = join[P + cidx];
+        if (sub == 0) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    dg[i][j] = join[(i * N + j) * TPR + t];
+                    db[i][j] = join[P + (i * N + j) * TPR + t];
+                }
         }
-    } else {
+    }
+    if (sub == 0) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            st<float, N>(out, (i * TPR + t) * N, C, dg[i]);
-            st<float, N>(out + C, (i * TPR + t) * N, C, db[i]);
+            if (skip[i] >= N) continue;
+            st<float, N>(out + at[i], dg[i]);
+            st<float, N>(out + C + at[i], db[i]);
         }
     }
 }
 
-// sums of the partial rows: 64 columns per workgroup, 16 waves share the rows (fixed assignment, fixed order of the join)
+// sums of the partial rows: 16 columns per workgroup, 64 groups of threads share the rows (fixed assignment, fixed order of the join)
 template <typename W>
 __global__ __launch_bounds__(1024) void layer_norm_wsum_kernel(const float* partial, int parts, int C, W* dgamma, W* dbeta) {
-    __shared__ float part[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = blockIdx.x * 64 + lane;
+    __shared__ float part[64][17];
+    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const int col = blockIdx.x * 16 + lane;
     float s = 0.f;
-    if (col < 2 * C)
-        for (int r = wave; r < parts; r += 16) s += partial[(long long)r * 2 * C + col];
-    part[wave][lane] = s;
-    __syncthreads();
-    if (wave || col >= 2 * C) return;
+    if (col < 2 * C) {
+        const float* p = partial + col;
+        int r = group;
+        for (; r + 7 * 64 < parts; r += 8 * 64) {          // eight loads under way at a time: this is a latency, not a bandwidth, problem
+            float v[8];
 #pragma unroll
-    for (int w = 1; w < 16; ++w) s += part[w][lane];
+            for (int k = 0; k < 8; ++k) v[k] = p[(long long)(r + k * 64) * 2 * C];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
+        for (; r < parts; r += 64) s += p[(long long)r * 2 * C];
+    }
+    part[group][lane] = s;
+    __syncthreads();
+    if (group >= 4) return;
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += part[group * 16 + w][lane];
+    s += __shfl_xor(s, 16, 64);                            // the four groups left are one wave
+    s += __shfl_xor(s, 32, 64);
     W* out = col < C ? dgamma : dbeta;
-    if (out) out[col < C ? col : col - C] = (W)s;
+    if (group == 0 && col < 2 * C && out) out[col < C ? col : col - C] = (W)s;
 }
 
 constexpr int MAX_C = 16384;
-constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024;      // persistent grids: 8 / 4 workgroups of 256 threads per CU
+// Persistent grids: 8 / 2 workgroups of 256 threads per CU.  Backward, 50 432 x 768 bf16 with an addend: 512 blocks 60.4 us, 768 64.3, 1024 73.4, 1536
+// 68.7 (5 003 x 1001 fp32: 16.3 / 20.4 / 21.5 / 25.1): every block leaves a partial row, and more than the registers hold at once run as a second, ragged wave of blocks.
+constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 512;
 
 struct Plan { int tpr, nc; };
-// a row on as few threads as hold it in 32 floats each: one wave up to 2048 columns (narrow rows share a wave), 256 threads up to 8192, else 1024
+// a row on as few threads as hold it in 32 floats each: one wave up to 2048 columns (narrow rows share a wave), 256 threads up to 8192, else 512
 Plan plan(int C, int n) {
-    const int vecs = (C + n - 1) / n;
+    const int vecs = C < n ? C : (C + n - 1) / n;        // rows shorter than a vector: element by element
     if (vecs <= 16) return {16, 1};
     if (vecs <= 32) return {32, 1};
     if (vecs <= 64) return {64, 1};
@@ -231,8 +290,7 @@ Plan plan(int C, int n) {
     if (vecs <= 512) return {256, 2};
     if (vecs <= 1024) return {256, 4};
     if (n == 4 && vecs <= 2048) return {256, 8};
-    if (vecs <= 2048) return {1024, 2};
-    return {1024, 4};
+    return {512, n == 4 ? 8 : 4};
 }
 int blocks_of(long long rows, const Plan& p, int most) {
     const int rpb = p.tpr >= 256 ? 1 : 256 / p.tpr;
@@ -242,35 +300,37 @@ int blocks_of(long long rows, const Plan& p, int most) {
 
 struct FwdCall {
     const void* x; long long rows; int C; long long xs; const void *gamma, *beta; float eps; void* y; long long ys; float* stats; hipStream_t s;
-    template <typename X, typename W, int TPR, int NC> void go() const {
-        hipLaunchKernelGGL((layer_norm_kernel<X, W, TPR, NC>), dim3(blocks_of(rows, {TPR, NC}, FWD_BLOCKS)), dim3(TPR > 256 ? TPR : 256), 0, s, (const X*)x, rows, C, xs,
+    template <typename X, typename W, int N, int TPR, int NC> void go() const {
+        hipLaunchKernelGGL((layer_norm_kernel<X, W, N, TPR, NC>), dim3(blocks_of(rows, {TPR, NC}, FWD_BLOCKS)), dim3(TPR > 256 ? TPR : 256), 0, s, (const X*)x, rows, C, xs,
                            (const W*)gamma, (const W*)beta, eps, (X*)y, ys, stats);
     }
 };
 struct BwdCall {
     const void* dy; long long dys; const void* x; long long xs, rows; int C; const void* gamma; const float* stats; const void* addend; long long as; void* dx; long long dxs;
     float* partial; hipStream_t s;
-    template <typename X, typename W, int TPR, int NC> void go() const {
-        hipLaunchKernelGGL((layer_norm_bwd_kernel<X, W, TPR, NC>), dim3(blocks_of(rows, {TPR, NC}, BWD_BLOCKS)), dim3(TPR > 256 ? TPR : 256), 0, s, (const X*)dy, dys,
+    template <typename X, typename W, int N, int TPR, int NC> void go() const {
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<X, W, N, TPR, NC>), dim3(blocks_of(rows, {TPR, NC}, BWD_BLOCKS)), dim3(TPR > 256 ? TPR : 256), 0, s, (const X*)dy, dys,
                            (const X*)x, xs, rows, C, (const W*)gamma, stats, (const X*)addend, as, (X*)dx, dxs, partial);
     }
 };
 template <typename X, typename W, typename Call>
 void dispatch(const Call& c, const Plan& p) {
-    if (p.tpr == 16) c.template go<X, W, 16, 1>();
-    else if (p.tpr == 32) c.template go<X, W, 32, 1>();
-    else if (p.tpr == 64 && p.nc == 1) c.template go<X, W, 64, 1>();
-    else if (p.tpr == 64 && p.nc == 2) c.template go<X, W, 64, 2>();
-    else if (p.tpr == 64 && p.nc == 3) c.template go<X, W, 64, 3>();
-    else if (p.tpr == 64 && p.nc == 4) c.template go<X, W, 64, 4>();
-    else if (p.tpr == 256 && p.nc == 4) c.template go<X, W, 256, 4>();
+    constexpr int N = 16 / sizeof(X);
+    if (c.C < N) c.template go<X, W, 1, 16, 1>();
+    else if (p.tpr == 16) c.template go<X, W, N, 16, 1>();
+    else if (p.tpr == 32) c.template go<X, W, N, 32, 1>();
+    else if (p.tpr == 64 && p.nc == 1) c.template go<X, W, N, 64, 1>();
+    else if (p.tpr == 64 && p.nc == 2) c.template go<X, W, N, 64, 2>();
+    else if (p.tpr == 64 && p.nc == 3) c.template go<X, W, N, 64, 3>();
+    else if (p.tpr == 64 && p.nc == 4) c.template go<X, W, N, 64, 4>();
+    else if (p.tpr == 256 && p.nc == 4) c.template go<X, W, N, 256, 4>();
     else if constexpr (sizeof(X) == 4) {
-        if (p.tpr == 64) c.template go<X, W, 64, 8>();
-        else if (p.tpr == 256) c.template go<X, W, 256, 8>();
-        else c.template go<X, W, 1024, 4>();
+        if (p.tpr == 64) c.template go<X, W, N, 64, 8>();
+        else if (p.tpr == 256) c.template go<X, W, N, 256, 8>();
+        else c.template go<X, W, N, 512, 8>();
     } else {
-        if (p.tpr == 256) c.template go<X, W, 256, 2>();
-        else c.template go<X, W, 1024, 2>();
+        if (p.tpr == 256) c.template go<X, W, N, 256, 2>();
+        else c.template go<X, W, N, 512, 4>();
     }
 }
 template <typename Call>
@@ -326,7 +386,7 @@ extern "C" int dp_layer_norm_bwd(const void* dy, long long dy_stride, const void
     DP_LAUNCH_CHECK("layer_norm_bwd");
     if (weights) {
         const int parts = blocks_of(rows, p, BWD_BLOCKS);
-        const dim3 grid((2 * C + 63) / 64);
+        const dim3 grid((2 * C + 15) / 16);
         if (w_dtype == 0) hipLaunchKernelGGL(layer_norm_wsum_kernel<float>, grid, dim3(1024), 0, s, (const float*)work, parts, C, (float*)dgamma, (float*)dbeta);
         else if (w_dtype == 1) hipLaunchKernelGGL(layer_norm_wsum_kernel<_Float16>, grid, dim3(1024), 0, s, (const float*)work, parts, C, (_Float16*)dgamma, (_Float16*)dbeta);
         else hipLaunchKernelGGL(layer_norm_wsum_kernel<__bf16>, grid, dim3(1024), 0, s, (const float*)work, parts, C, (__bf16*)dgamma, (__bf16*)dbeta);
