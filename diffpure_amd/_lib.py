@@ -62,15 +62,16 @@ SIGNATURES = {
     "dp_timestep_embedding": [_p, _i, _p, _i, _i, _p, _p],
     "dp_em_step": [_p, _p, _i, _i, _i, _i, _f, _f, _f, _i, _f, _f, _f, _p, _ull, _ll, _i, _p, _p],
     "dp_philox_normal": [_p, _i, _ll, _ull, _ll, _i, _p],
-    "dp_attention_lse": [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _f, _i, _p, _p, _p],
-    "dp_attention_lse_bwd_workspace": [_i, _i, _i],
+    "dp_attention_lse": [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _f, _i, _p, _p, _p, _ll, _p],
+    "dp_attention_lse_workspace": [_i, _i, _i, _i, _i, _i, _i],
+    "dp_attention_lse_bwd_workspace": [_i, _i, _i, _i, _i, _i, _i],
     "dp_attention_lse_bwd": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _f, _i, _p, _p, _p, _p, _ll, _p],
     "dp_layer_norm": [_p, _i, _ll, _i, _ll, _p, _p, _i, _f, _p, _ll, _p, _p],
     "dp_layer_norm_bwd_workspace": [_ll, _i, _i],
     "dp_layer_norm_bwd": [_p, _ll, _p, _ll, _i, _ll, _i, _p, _i, _p, _p, _ll, _p, _ll, _p, _p, _p, _ll, _p],
     "dp_ddpm_step": [_p, _p, _i, _i, _i, _f, _f, _f, _f, _f, _f, _i, _p, _ull, _ll, _i, _p, _p],
 }
-_RESTYPE = {"dp_last_error": C.c_char_p, "dp_conv2d_nhwc_h2_workspace": C.c_longlong, "dp_attention_lse_bwd_workspace": C.c_longlong,
+_RESTYPE = {"dp_last_error": C.c_char_p, "dp_conv2d_nhwc_h2_workspace": C.c_longlong, "dp_attention_lse_workspace": C.c_longlong, "dp_attention_lse_bwd_workspace": C.c_longlong,
             "dp_layer_norm_bwd_workspace": C.c_longlong}
 
 _lib = None

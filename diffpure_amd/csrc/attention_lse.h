@@ -86,14 +86,18 @@ __device__ __forceinline__ typename Tr<DT>::Frag pack(const typename Tr<DT>::Acc
     }
 }
 
-// LDS image of a streamed tile: rows of RB bytes, the 16-byte slots of a row XOR-ed with the row so that the lanes of a read (one slot of
-// many rows, or two slots of four rows in the transposing read) fall on different banks.  SWM + 1 divides the slots of a row.
-template <int RB> struct Lds {
+// LDS image of a streamed tile: rows of RB bytes, the 16-byte slots of a row XOR-ed with bits of the row.  The 64 banks take 16 slots at a time, so
+//   - a row read (one slot of 16 consecutive rows) wants 16 different places for the rows, and
+//   - a transposing read (4 slots of 4 rows: consecutive ones for 16-bit types, 4 apart in fp32) wants the four rows in different groups of 4 slots.
+// Rows of 256 bytes and more: the row bits that such a read runs over go to the upper two bits of the XOR, the other two to the lower ones.  Shorter rows
+// already differ by their start; the remaining row bits go the same way.  (Rows of 128 bytes in fp32 keep a two-way conflict in the transposing read.)
+template <int RB, int ES> struct Lds {
     static constexpr int SLOTS = RB / 16;
-    static constexpr int POW2 = SLOTS & -SLOTS;
-    static constexpr int SWM = (POW2 < 8 ? POW2 : 8) - 1;
-    // rows of 64 bytes: four of them span the banks, so the XOR takes the row's upper bits
-    static __device__ __forceinline__ int swz(int row) { return SLOTS == 4 ? (row >> 2) & SWM : row & SWM; }
+    static __device__ __forceinline__ int swz(int row) {
+        if constexpr (SLOTS % 16 == 0) return ES == 4 ? row & 15 : ((row & 3) << 2) | ((row >> 2) & 3);
+        else if constexpr (SLOTS % 8 == 0) return ES == 4 ? (row >> 1) & 7 : ((row & 2) << 1) | ((row >> 2) & 3);
+        else return (row >> 2) & 3;
+    }
     static __device__ __forceinline__ int at(int row, int slot) { return row * RB + ((slot ^ swz(row)) << 4); }
 };
 
@@ -101,7 +105,7 @@ template <int RB> struct Lds {
 template <int DT, int RB>
 __device__ __forceinline__ typename Tr<DT>::Frag ld_row(const char* tile, int lane, int ks) {
     using T = Tr<DT>;
-    return *reinterpret_cast<const typename T::Frag*>(tile + Lds<RB>::at(lane & (T::TILE - 1), ks * T::G + lane / T::TILE));
+    return *reinterpret_cast<const typename T::Frag*>(tile + Lds<RB, T::ES>::at(lane & (T::TILE - 1), ks * T::G + lane / T::TILE));
 }
 
 // A operand, transposed: row = d of block dt, k = the 16 streamed rows of step kk in the accumulator's order
@@ -113,14 +117,14 @@ __device__ __forceinline__ typename Tr<DT>::Frag ld_tr(const char* tile, int lan
     if constexpr (DT == 0) {
         const int byte = (dt * 16 + (lane & 15)) * 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(tile + Lds<RB>::at(4 * g + j, byte >> 4) + (byte & 12));
+        for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(tile + Lds<RB, T::ES>::at(4 * g + j, byte >> 4) + (byte & 12));
     } else {
         const int i = lane & 15, byte = (dt * 32 + (lane & 16) + 4 * (i & 3)) * 2;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int row = kk * 16 + half * 8 + 4 * g + (i >> 2);
             const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(tile + Lds<RB>::at(row, byte >> 4) + (byte & 8)));
+                (__attribute__((address_space(3))) s16x4*)(tile + Lds<RB, T::ES>::at(row, byte >> 4) + (byte & 8)));
             const typename T::E4 e = __builtin_bit_cast(typename T::E4, v);
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[half * 4 + j] = e[j];
@@ -129,39 +133,42 @@ __device__ __forceinline__ typename Tr<DT>::Frag ld_tr(const char* tile, int lan
     return f;
 }
 
-#define AL_GLDS(src, dst)                                                                      \
+#define AL_GLDS(src, dst, bytes)                                                               \
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src),     \
-                                     (__attribute__((address_space(3))) void*)(dst), 16, 0, 0)
+                                     (__attribute__((address_space(3))) void*)(dst), bytes, 0, 0)
 
-// Streams BM rows of two matrices into LDS (asynchronous copies, 1 KB per wave and instruction).  Rows behind the last one are read from
-// the last one and slots behind the head dimension from its last slot: the copies stay inside the tensors and bring in finite values,
-// which the masks (rows) and the zeroed kept operand (slots) take out again.
-template <int RB, int BM, int NW> struct Stream {
+// Streams BM rows of two matrices into LDS (asynchronous copies, 1 KB per wave and instruction): a uniform base that walks down the rows and 32-bit
+// offsets per lane.  In the last tile, rows behind the last one are read from the last one, and slots behind the head dimension always from its last
+// slot: the copies stay inside the tensors and bring in finite values, which the masks (rows) and the zeroed kept operand (slots) take out again.
+template <int RB, int ES, int BM, int NW> struct Stream {
     static constexpr int TILE_BYTES = BM * RB, STAGE = 2 * TILE_BYTES, PIECES = STAGE / (1024 * NW);
     static_assert(TILE_BYTES % 1024 == 0 && STAGE % (1024 * NW) == 0, "a wave's copy lies in one matrix, and the waves share the copies evenly");
-    const char* base[PIECES];
-    long long stride[PIECES];
-    int row[PIECES];
+    using L = Lds<RB, ES>;
+    const char *x0, *x1;                // row 0 of the two matrices
+    long long s0, s1;                   // bytes per row (at most 2^24: BM rows stay within 32 bits)
+    unsigned off[PIECES];
+    int row_slots, wave, lane;
 
-    __device__ __forceinline__ void init(const char* x0, long long s0, const char* x1, long long s1, int row_slots, int wave, int lane) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int byte = (i * NW + wave) * 1024;
-            const bool second = byte >= TILE_BYTES;
-            const int id = ((byte - (second ? TILE_BYTES : 0)) >> 4) + lane;
-            row[i] = id / Lds<RB>::SLOTS;
-            const int slot = (id % Lds<RB>::SLOTS) ^ Lds<RB>::swz(row[i]);
-            base[i] = (second ? x1 : x0) + (slot < row_slots ? slot : row_slots - 1) * 16;
-            stride[i] = second ? s1 : s0;
-        }
+    __device__ __forceinline__ bool second(int i) const { return (i * NW + wave) * 1024 >= TILE_BYTES; }
+    __device__ __forceinline__ int slot_id(int i) const { return (((i * NW + wave) * 1024 - (second(i) ? TILE_BYTES : 0)) >> 4) + lane; }
+    __device__ __forceinline__ unsigned offset(int i, int rows) const {       // rows: how many there are from the tile's first on
+        const int id = slot_id(i), row = id / L::SLOTS, slot = (id % L::SLOTS) ^ L::swz(row);
+        return (unsigned)(row < rows ? row : rows - 1) * (unsigned)(second(i) ? s1 : s0) + (slot < row_slots ? slot : row_slots - 1) * 16;
     }
-    // rows r0 .. r0 + BM - 1 (n > 0 rows exist) of the matrices moved by o0 / o1 bytes
-    __device__ __forceinline__ void issue(char* stage, int r0, int n, long long o0, long long o1, int wave) const {
+    __device__ __forceinline__ void init(const char* x0_, long long s0_, const char* x1_, long long s1_, int row_slots_, int wave_, int lane_) {
+        x0 = x0_; x1 = x1_; s0 = s0_; s1 = s1_; row_slots = row_slots_; wave = wave_; lane = lane_;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const bool second = (i * NW + wave) * 1024 >= TILE_BYTES;
-            const int r = r0 + row[i] < n ? r0 + row[i] : n - 1;
-            AL_GLDS(base[i] + (second ? o1 : o0) + (long long)r * stride[i], stage + (i * NW + wave) * 1024);
+        for (int i = 0; i < PIECES; ++i) off[i] = offset(i, BM);
+    }
+    // rows r0 .. r0 + BM - 1 of n (r0 < n) of the matrices moved by o0 / o1 bytes
+    __device__ __forceinline__ void issue(char* stage, int r0, int n, long long o0, long long o1) const {
+        const char *b0 = x0 + o0 + r0 * s0, *b1 = x1 + o1 + r0 * s1;
+        if (r0 + BM <= n) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) AL_GLDS((second(i) ? b1 : b0) + off[i], stage + (i * NW + wave) * 1024, 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) AL_GLDS((second(i) ? b1 : b0) + offset(i, n - r0), stage + (i * NW + wave) * 1024, 16);
         }
     }
 };
@@ -183,16 +190,25 @@ __device__ __forceinline__ int clamp_len(const int* lens, int b, int t) {
     return n < 0 ? 0 : (n > t ? t : n);
 }
 
-// reduction over the lane groups that share a column
-template <int TILE> __device__ __forceinline__ float col_sum(float v) {
-#pragma unroll
-    for (int o = TILE; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+// reductions over the lane groups that share a column (lane ^ 32; fp32 tiles of 16 also lane ^ 16): register swaps, no LDS
+template <int TILE, typename F> __device__ __forceinline__ float col_reduce(float v, F f) {
+    const unsigned u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned lo = r[0], hi = r[1];
+    v = f(__uint_as_float(lo), __uint_as_float(hi));
+    if constexpr (TILE == 16) {
+        const unsigned w = __float_as_uint(v);
+        const auto q = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+        const unsigned a = q[0], b = q[1];
+        v = f(__uint_as_float(a), __uint_as_float(b));
+    }
     return v;
 }
+template <int TILE> __device__ __forceinline__ float col_sum(float v) {
+    return col_reduce<TILE>(v, [](float a, float b) { return a + b; });
+}
 template <int TILE> __device__ __forceinline__ float col_max(float v) {
-#pragma unroll
-    for (int o = TILE; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    return col_reduce<TILE>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // kept operand: 16 bytes per step of one row of a tensor, slots behind the head dimension zero
@@ -208,20 +224,43 @@ __device__ __forceinline__ void ld_kept(typename Tr<DT>::Frag (&f)[KS], const ch
     }
 }
 
-// one kept column of an accumulator block [d][column], times `mul`, to a row of D elements
-template <int DT, int ND>
-__device__ __forceinline__ void st_col(const typename Tr<DT>::Acc (&acc)[ND], float mul, char* rowp, int D, int g) {
+// An accumulator block [d][column] is stored in units of four consecutive d: unit u = block dt, registers 4 i .. 4 i + 3.
+template <int DT, int ND> struct Units {
     using T = Tr<DT>;
+    static constexpr int PER = T::NR / 4, N = ND * PER;
+    static __device__ __forceinline__ int d(int u, int g) { return (u / PER) * T::TILE + (u % PER) * 4 * T::G + 4 * g; }
+    static __device__ __forceinline__ f32x4 get(const typename T::Acc (&acc)[ND], int u) {
+        const int r = (u % PER) * 4;
+        return f32x4{acc[u / PER][r], acc[u / PER][r + 1], acc[u / PER][r + 2], acc[u / PER][r + 3]};
+    }
+};
+template <int DT> __device__ __forceinline__ void st4(char* rowp, int d, f32x4 v) {
+    typename Tr<DT>::E4 e;
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt)
+    for (int j = 0; j < 4; ++j) e[j] = (typename Tr<DT>::E)v[j];
+    *reinterpret_cast<typename Tr<DT>::E4*>(rowp + (long long)d * Tr<DT>::ES) = e;
+}
+// The waves that took different rows for the same columns (RS of them, rank rw) join their accumulators: every wave leaves its units in LDS and sums a
+// share of them, in the order of the ranks.  sink(unit, sum) gets each unit once.  smem: Units::N KB per wave; a barrier must lie before the call.
+template <int DT, int ND, int RS, typename Sink>
+__device__ __forceinline__ void join_units(const typename Tr<DT>::Acc (&acc)[ND], float mul, char* smem, int wave, int rw, int lane, Sink sink) {
+    using U = Units<DT, ND>;
+    if constexpr (RS == 1) {
 #pragma unroll
-        for (int r = 0; r < T::NR; r += 4) {
-            const int d = dt * T::TILE + r * T::G + 4 * g;
-            typename T::E4 v;
+        for (int u = 0; u < U::N; ++u) sink(u, U::get(acc, u) * mul);
+    } else {
+        f32x4* mine = reinterpret_cast<f32x4*>(smem) + (long long)wave * U::N * 64 + lane;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = (typename T::E)(acc[dt][r + j] * mul);
-            if (d < D) *reinterpret_cast<typename T::E4*>(rowp + (long long)d * T::ES) = v;
+        for (int u = 0; u < U::N; ++u) mine[u * 64] = U::get(acc, u) * mul;
+        __syncthreads();
+        const f32x4* first = reinterpret_cast<const f32x4*>(smem) + (long long)(wave - rw) * U::N * 64 + lane;
+        for (int u = rw; u < U::N; u += RS) {
+            f32x4 s = first[u * 64];
+#pragma unroll
+            for (int w = 1; w < RS; ++w) s += first[(w * U::N + u) * 64];
+            sink(u, s);
         }
+    }
 }
 
 // row of the tile that register r holds (plus 4 g)
@@ -237,12 +276,108 @@ struct Args {
     Ten q, k, v, o, dout;         // out / dout: backward only
     Ten w0, w1;                   // what the kernel writes: out (forward), dq, or dk and dv
     float* lse;                   // [B, Hq, Tq]
-    float* ws;                    // backward: [2][B, Hq, Tqp] log2-domain log-sum-exp (+inf: no such row) and delta; forward: see there
+    float* rows;                  // backward: [2][B, Hq, Tqp] log2-domain log-sum-exp (+inf: no such row) and -delta
+    float *part0, *part1;         // split launches: partial results, [split][kept row][D] (the order of kept rows: see Kept)
+    float* part_lse;              // forward: [split][kept row]
     const int *q_lens, *kv_lens;
     int B, Tq, Tk, Hq, Hkv, D, Tqp;
+    int packed;                   // 1: the queries of all heads of a group are the columns of one block (heads share their keys)
+    int splits, split_rows;       // the streamed rows are cut into `splits` ranges of split_rows
     float scale;
     int causal, xcd_map;
 };
+
+// The kept queries of a workgroup.  Not packed: z = one query head, column = token.  Packed: z = one key head, column = head of the group * Tq + token.
+struct Kept {
+    int b, hk, h0, cols;
+    __device__ __forceinline__ Kept(const Args& p, int z) {
+        const int heads = p.packed ? p.Hkv : p.Hq;
+        b = z / heads;
+        const int h = z - b * heads, group = p.Hq / p.Hkv;
+        hk = p.packed ? h : h / group;
+        h0 = p.packed ? h * group : h;
+        cols = p.packed ? group * p.Tq : p.Tq;
+    }
+    __device__ __forceinline__ void col(const Args& p, int c, int& h, int& t) const {
+        const int i = p.packed ? c / p.Tq : 0;
+        h = h0 + i;
+        t = c - i * p.Tq;
+    }
+};
+
+}  // namespace al
+
+namespace al {
+
+inline int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
+
+// How a launch that keeps queries (forward, dQ) covers the chip of 256 CUs.
+//   packed: heads that share their keys are columns of one block where all their queries fit two tiles (a key is then read once per group).
+//   rs:     waves of a workgroup that share one tile of columns and divide the streamed rows (1: every wave has its own columns).  Sharing makes
+//           four times the workgroups with a quarter of the rows each.
+//   splits: ranges of the streamed rows that workgroups of their own take, joined by a second launch.
+struct QPlan {
+    int packed, rs, splits, split_rows;
+    long long blocks;
+};
+inline QPlan q_plan(int B, int Tq, int Tk, int Hq, int Hkv, int DP, int tile) {
+    QPlan pl;
+    const int group = Hq / Hkv;
+    pl.packed = group > 1 && (long long)group * Tq <= 2 * tile;
+    const long long heads = (long long)B * (pl.packed ? Hkv : Hq), cols = pl.packed ? (long long)group * Tq : Tq;
+    pl.rs = 1;
+    pl.blocks = heads * ((cols + 4 * tile - 1) / (4 * tile));
+    if (cols <= tile || pl.blocks < 256) {
+        pl.rs = DP > 128 ? 2 : 4;
+        const int wide = tile * 4 / pl.rs;
+        pl.blocks = heads * ((cols + wide - 1) / wide);
+    }
+    pl.splits = 1;
+    const int stage = pl.rs * tile;
+    if (pl.blocks < 256) {
+        const long long want = (512 + pl.blocks - 1) / pl.blocks, most = Tk / (4 * stage);
+        pl.splits = (int)(want < most ? want : most);
+        if (pl.splits < 1) pl.splits = 1;
+        if (pl.splits > 128) pl.splits = 128;
+    }
+    const int stages = (Tk + stage - 1) / stage;
+    pl.split_rows = (stages + pl.splits - 1) / pl.splits * stage;
+    pl.splits = (Tk + pl.split_rows - 1) / pl.split_rows;
+    return pl;
+}
+
+// The same for the launch that keeps keys (dK, dV).  Its partial sums are as large as 2 * splits results, so it is split for causal launches (whose
+// blocks differ in length) and for those that would leave CUs without a workgroup.
+struct KPlan {
+    int rs, splits, split_rows;
+    long long blocks;
+};
+inline KPlan k_plan(int B, int Tq, int Tk, int Hq, int Hkv, int D, int DP, int tile, bool f32, int causal) {
+    (void)D;
+    (void)Hq;
+    KPlan pl;
+    const long long heads = (long long)B * Hkv;
+    pl.rs = 1;
+    pl.blocks = heads * ((Tk + 4LL * tile - 1) / (4 * tile));
+    if (pl.blocks < 256) {
+        pl.rs = DP > 128 ? 2 : 4;
+        const int wide = tile * 4 / pl.rs;
+        pl.blocks = heads * ((Tk + wide - 1) / wide);
+    }
+    const int stage = pl.rs > 1 ? pl.rs * tile : (f32 ? 2 : 1) * tile;
+    pl.splits = 1;
+    const long long enough = causal ? 1024 : 256;
+    if (pl.blocks < enough) {
+        const long long want = ((causal ? 1024 : 512) + pl.blocks - 1) / pl.blocks, most = Tq / (4 * stage);
+        pl.splits = (int)(want < most ? want : most);
+        if (pl.splits < 1) pl.splits = 1;
+        if (pl.splits > 64) pl.splits = 64;
+    }
+    const int stages = (Tq + stage - 1) / stage;
+    pl.split_rows = (stages + pl.splits - 1) / pl.splits * stage;
+    pl.splits = (Tq + pl.split_rows - 1) / pl.split_rows;
+    return pl;
+}
 
 }  // namespace al
 

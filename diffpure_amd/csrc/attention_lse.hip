@@ -5,31 +5,37 @@
 namespace {
 using namespace al;
 
-// One workgroup = 4 waves, each CW tiles of query columns; K and V tiles of TILE rows stream through LDS (double buffered).
+// One workgroup = 4 waves; K and V tiles stream through LDS (double buffered).  RS = 1: every wave has its own CW tiles of query columns and sees every
+// streamed row.  RS > 1 (few columns): RS waves share their columns and take different rows of a stage; they join at the end.
 // The running maximum is only moved when a row's maximum has grown by more than 8 (in log2): until then the probabilities are taken
 // against the old one - at most 2^8, exact in every type's range - and neither sum nor output is rescaled.
-template <int DT, int DP, int CW>
-__global__ __launch_bounds__(256) AL_WAVES(DP <= 128 ? 2 : 1) void attn_lse_fwd_kernel(Args p) {
+template <int DT, int DP, int CW, int RS, int RT>
+__global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_fwd_kernel(Args p) {
     using T = Tr<DT>;
-    constexpr int NW = 4, BM = T::TILE, RB = DP * T::ES, KS = DP / 16, ND = DP / T::TILE, NKK = T::TILE / 16, COLS = NW * CW * T::TILE;
-    using St = Stream<RB, BM, NW>;
+    constexpr int NW = 4, BM = RS * RT * T::TILE, RB = DP * T::ES, KS = DP / 16, ND = DP / T::TILE, NKK = T::TILE / 16, COLS = NW / RS * CW * T::TILE;
+    using St = Stream<RB, T::ES, BM, NW>;
     __shared__ __attribute__((aligned(1024))) char smem[2 * St::STAGE];
+    __shared__ float ml[RS > 1 ? 2 : 1][NW][CW * T::TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cl = lane & (T::TILE - 1), g = lane / T::TILE;
-    const int nblk = (p.Tq + COLS - 1) / COLS;
-    const int bid = logical_block(p.xcd_map);
+    const int rw = wave % RS, cl = lane & (T::TILE - 1), g = lane / T::TILE;
+    const int bid0 = logical_block(p.xcd_map), split = bid0 % p.splits, bid = bid0 / p.splits;
+    const int cols0 = p.packed ? p.Hq / p.Hkv * p.Tq : p.Tq, nblk = (cols0 + COLS - 1) / COLS;
     const int z = bid / nblk, blk = p.causal ? nblk - 1 - (bid - z * nblk) : bid - z * nblk;     // causal: the long blocks first
-    const int b = z / p.Hq, h = z - b * p.Hq, hk = h / (p.Hq / p.Hkv);
+    const Kept kept(p, z);
+    const int b = kept.b;
     const int n = clamp_len(p.q_lens, b, p.Tq), m = clamp_len(p.kv_lens, b, p.Tk), off = m - n;
-    const int c0 = blk * COLS, wc0 = c0 + wave * CW * T::TILE;       // first column of the workgroup / of this wave
+    const int c0 = blk * COLS, wc0 = c0 + wave / RS * CW * T::TILE;       // first column of the workgroup / of this wave
     const int row_slots = p.D * T::ES / 16;
     const float c = fabsf(p.scale) * LOG2E;
 
     typename T::Frag qf[CW][KS];
+    int head[CW], tok[CW];
 #pragma unroll
     for (int cw = 0; cw < CW; ++cw) {
-        const int col = wc0 + cw * T::TILE + cl, row = col < n ? col : (n > 0 ? n - 1 : 0);
-        ld_kept<DT, KS>(qf[cw], p.q.p + b * p.q.b + h * p.q.h + (long long)row * p.q.t, row_slots, g);
+        const int col = wc0 + cw * T::TILE + cl;
+        kept.col(p, col < kept.cols ? col : kept.cols - 1, head[cw], tok[cw]);
+        const int row = tok[cw] < n ? tok[cw] : (n > 0 ? n - 1 : 0);
+        ld_kept<DT, KS>(qf[cw], p.q.p + b * p.q.b + head[cw] * p.q.h + row * p.q.t, row_slots, g);
         if (p.scale < 0.f) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) qf[cw][ks] = -qf[cw][ks];
@@ -45,105 +51,167 @@ __global__ __launch_bounds__(256) AL_WAVES(DP <= 128 ? 2 : 1) void attn_lse_fwd_
         for (int dt = 0; dt < ND; ++dt) o[cw][dt] = typename T::Acc{};
     }
 
-    int rows_end = c0 < n ? m : 0;
-    if (p.causal) {
-        const int last = (c0 + COLS < n ? c0 + COLS : n) - 1 + off;      // last key of the last query
-        rows_end = last + 1 < rows_end ? last + 1 : rows_end;
-    }
+    // streamed rows: [begin, open) are seen by every column, [open, end) through the mask
+    const int t0 = p.packed ? 0 : c0, t1 = p.packed ? p.Tq : c0 + COLS;
+    int begin = split * p.split_rows, end = t0 < n ? m : 0, open;
+    if (p.causal) end = min(end, min(t1, n) + off);
+    end = min(end, begin + p.split_rows);
+    open = p.causal ? min(end, t0 + off + 1) : end;
+    open = begin + max(open - begin, 0) / BM * BM;
     St st;
-    st.init(p.k.p + b * p.k.b + hk * p.k.h, p.k.t, p.v.p + b * p.v.b + hk * p.v.h, p.v.t, row_slots, wave, lane);
-    if (rows_end > 0) st.issue(smem, 0, m, 0, 0, wave);
+    st.init(p.k.p + b * p.k.b + kept.hk * p.k.h, p.k.t, p.v.p + b * p.v.b + kept.hk * p.v.h, p.v.t, row_slots, wave, lane);
+    if (begin < end) st.issue(smem, begin, m, 0, 0);
     int cur = 0;
-    for (int r0 = 0; r0 < rows_end; r0 += BM, cur ^= 1) {
+    auto body = [&](int r0, auto masked) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (r0 + BM < rows_end) st.issue(smem + (cur ^ 1) * St::STAGE, r0 + BM, m, 0, 0, wave);
-        const char* Ks = smem + cur * St::STAGE;
-        const char* Vs = Ks + St::TILE_BYTES;
-        auto tile = [&](auto masked) {
-        typename T::Acc s[CW];
+        if (r0 + BM < end) st.issue(smem + (cur ^ 1) * St::STAGE, r0 + BM, m, 0, 0);
+        const char* stage = smem + cur * St::STAGE;
+        cur ^= 1;
 #pragma unroll
-        for (int cw = 0; cw < CW; ++cw) s[cw] = typename T::Acc{};
+        for (int rt = 0; rt < RT; ++rt) {
+            const int rr = (rw * RT + rt) * T::TILE;
+            const char *Ks = stage + rr * RB, *Vs = Ks + St::TILE_BYTES;
+            typename T::Acc s[CW];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const typename T::Frag a = ld_row<DT, RB>(Ks, lane, ks);
+            for (int cw = 0; cw < CW; ++cw) s[cw] = typename T::Acc{};
 #pragma unroll
-            for (int cw = 0; cw < CW; ++cw) s[cw] = T::mma(a, qf[cw][ks], s[cw]);
-        }
-        if constexpr (masked.value) {
+            for (int ks = 0; ks < KS; ++ks) {
+                const typename T::Frag a = ld_row<DT, RB>(Ks, lane, ks);
+#pragma unroll
+                for (int cw = 0; cw < CW; ++cw) s[cw] = T::mma(a, qf[cw][ks], s[cw]);
+            }
+            if constexpr (masked.value) {
+#pragma unroll
+                for (int cw = 0; cw < CW; ++cw) {
+                    const int seen = min(end, p.causal ? tok[cw] + off + 1 : end) - r0 - rr - 4 * g;
+#pragma unroll
+                    for (int r = 0; r < T::NR; ++r) s[cw][r] = reg_row<DT>(r) < seen ? s[cw][r] : -INFINITY;
+                }
+            }
 #pragma unroll
             for (int cw = 0; cw < CW; ++cw) {
-                int end = p.causal ? wc0 + cw * T::TILE + cl + off + 1 : m;
-                end = (end < m ? end : m) - r0 - 4 * g;
+                float mb = s[cw][0];
 #pragma unroll
-                for (int r = 0; r < T::NR; ++r) s[cw][r] = reg_row<DT>(r) < end ? s[cw][r] : -INFINITY;
+                for (int r = 1; r < T::NR; ++r) mb = fmaxf(mb, s[cw][r]);
+                mb = col_max<T::TILE>(mb);
+                const bool grow = mb * c > mx[cw] * c + 8.f;
+                if (__any(grow)) {
+                    const float nm = grow ? mb : mx[cw];
+                    const float alpha = mx[cw] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx[cw] - nm) * c);
+                    mx[cw] = nm;
+                    l[cw] *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                        for (int r = 0; r < T::NR; ++r) o[cw][dt][r] *= alpha;
+                }
+                const float mc = mx[cw] == -INFINITY ? 0.f : mx[cw] * c;
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < T::NR; ++r) {
+                    s[cw][r] = __builtin_amdgcn_exp2f(fmaf(s[cw][r], c, -mc));
+                    sum += s[cw][r];
+                }
+                l[cw] += sum;
             }
-        }
 #pragma unroll
-        for (int cw = 0; cw < CW; ++cw) {
-            float mb = s[cw][0];
+            for (int kk = 0; kk < NKK; ++kk) {
+                typename T::Frag pf[CW];
 #pragma unroll
-            for (int r = 1; r < T::NR; ++r) mb = fmaxf(mb, s[cw][r]);
-            mb = col_max<T::TILE>(mb);
-            const bool grow = mb * c > mx[cw] * c + 8.f;
-            if (__any(grow)) {
-                const float nm = grow ? mb : mx[cw];
-                const float alpha = mx[cw] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx[cw] - nm) * c);
-                mx[cw] = nm;
-                l[cw] *= alpha;
+                for (int cw = 0; cw < CW; ++cw) pf[cw] = pack<DT>(s[cw], kk);
 #pragma unroll
-                for (int dt = 0; dt < ND; ++dt)
+                for (int dt = 0; dt < ND; ++dt) {
+                    const typename T::Frag a = ld_tr<DT, RB>(Vs, lane, kk, dt);
 #pragma unroll
-                    for (int r = 0; r < T::NR; ++r) o[cw][dt][r] *= alpha;
-            }
-            const float mc = mx[cw] == -INFINITY ? 0.f : mx[cw] * c;
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < T::NR; ++r) {
-                s[cw][r] = __builtin_amdgcn_exp2f(fmaf(s[cw][r], c, -mc));
-                sum += s[cw][r];
-            }
-            l[cw] += sum;
-        }
-#pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) {
-            typename T::Frag pf[CW];
-#pragma unroll
-            for (int cw = 0; cw < CW; ++cw) pf[cw] = pack<DT>(s[cw], kk);
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) {
-                const typename T::Frag a = ld_tr<DT, RB>(Vs, lane, kk, dt);
-#pragma unroll
-                for (int cw = 0; cw < CW; ++cw) o[cw][dt] = T::mma(a, pf[cw], o[cw][dt]);
+                    for (int cw = 0; cw < CW; ++cw) o[cw][dt] = T::mma(a, pf[cw], o[cw][dt]);
+                }
             }
         }
         settle();
-        };
-        if (p.causal && r0 > wc0 + CW * T::TILE - 1 + off) {}            // every key of the tile lies behind this wave's queries
-        else if (r0 + BM > m || (p.causal && r0 + BM - 1 > wc0 + off)) tile(yes{});
-        else tile(no{});
-    }
+    };
+    int r0 = begin;
+    for (; r0 < open; r0 += BM) body(r0, no{});
+    for (; r0 < end; r0 += BM) body(r0, yes{});
 
+    if constexpr (RS > 1) __syncthreads();
 #pragma unroll
     for (int cw = 0; cw < CW; ++cw) {
         const int col = wc0 + cw * T::TILE + cl;
-        const float sum = col_sum<T::TILE>(l[cw]);
-        if (col >= p.Tq) continue;
-        const bool some = col < n && sum > 0.f;
-        if (!some) {
+        float sum = col_sum<T::TILE>(l[cw]), top = mx[cw], mine = 1.f;
+        if constexpr (RS > 1) {
+            if (g == 0) {
+                ml[0][wave][cw * T::TILE + cl] = top;
+                ml[1][wave][cw * T::TILE + cl] = sum;
+            }
+            __syncthreads();
 #pragma unroll
-            for (int dt = 0; dt < ND; ++dt) o[cw][dt] = typename T::Acc{};
+            for (int w = 0; w < RS; ++w) top = fmaxf(top, ml[0][wave - rw + w][cw * T::TILE + cl]);
+            const float tc = top == -INFINITY ? 0.f : top * c;
+            mine = __builtin_amdgcn_exp2f(mx[cw] * c - tc);
+            sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < RS; ++w) sum += ml[1][wave - rw + w][cw * T::TILE + cl] * __builtin_amdgcn_exp2f(ml[0][wave - rw + w][cw * T::TILE + cl] * c - tc);
         }
-        st_col<DT, ND>(o[cw], some ? 1.f / sum : 0.f, const_cast<char*>(p.w0.p) + b * p.w0.b + h * p.w0.h + (long long)col * p.w0.t, p.D, g);
-        if (g == 0) p.lse[(long long)z * p.Tq + col] = some ? mx[cw] * fabsf(p.scale) + logf(sum) : -INFINITY;
+        const bool some = tok[cw] < n && sum > 0.f;
+        const float inv = some ? 1.f / sum : 0.f, lse = some ? top * fabsf(p.scale) + logf(sum) : -INFINITY;
+        const bool out = col < kept.cols;
+        const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
+        char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head[cw] * p.w0.h + tok[cw] * p.w0.t;
+        join_units<DT, ND, RS>(o[cw], mine, smem, wave, rw, lane, [&](int u, f32x4 v) {
+            const int d = Units<DT, ND>::d(u, g);
+            if (!out || d >= p.D) return;
+            v = some ? v * inv : f32x4{};
+            if (p.splits > 1) *reinterpret_cast<f32x4*>(p.part0 + kr * p.D + d) = v;
+            else st4<DT>(row, d, v);
+        });
+        if (out && g == 0 && rw == 0) {
+            if (p.splits > 1) p.part_lse[kr] = lse;
+            else p.lse[((long long)b * p.Hq + head[cw]) * p.Tq + tok[cw]] = lse;
+        }
+        if constexpr (RS > 1 && CW > 1) __syncthreads();
     }
 }
 
+// joins the ranges of a split launch: out = sum_s 2^(lse_s - lse) out_s.  One thread per four channels of a kept row.
+template <int DT>
+__global__ __launch_bounds__(256) void attn_lse_join_kernel(Args p) {
+    const int per = p.D / 4, heads = p.packed ? p.Hkv : p.Hq, cols = p.packed ? p.Hq / p.Hkv * p.Tq : p.Tq;
+    const long long rows = (long long)p.B * heads * cols, id = (long long)blockIdx.x * 256 + threadIdx.x, kr = id / per;
+    const int d = (int)(id - kr * per) * 4;
+    if (kr >= rows) return;
+    const int z = (int)(kr / cols);
+    const Kept kept(p, z);
+    int h, t;
+    kept.col(p, (int)(kr - (long long)z * cols), h, t);
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[s * rows + kr]);
+    f32x4 v = {};
+    if (top > -INFINITY) {
+        for (int s = 0; s < p.splits; ++s) {
+            const float w = __builtin_amdgcn_exp2f((p.part_lse[s * rows + kr] - top) * LOG2E);
+            sum += w;
+            v += w * *reinterpret_cast<const f32x4*>(p.part0 + (s * rows + kr) * p.D + d);
+        }
+        v *= 1.f / sum;
+    }
+    st4<DT>(const_cast<char*>(p.w0.p) + kept.b * p.w0.b + h * p.w0.h + t * p.w0.t, d, v);
+    if (d == 0) p.lse[((long long)kept.b * p.Hq + h) * p.Tq + t] = top > -INFINITY ? top + logf(sum) : -INFINITY;
+}
+
 template <int DT, int DP>
-void launch_fwd(const Args& a, hipStream_t s) {
-    constexpr int COLS = 4 * Tr<DT>::TILE;
-    const long long blocks = (long long)a.B * a.Hq * ((a.Tq + COLS - 1) / COLS);
-    hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+void launch_fwd(Args a, hipStream_t s) {
+    constexpr int TILE = Tr<DT>::TILE, WIDE = DP > 128 ? 2 : 4;
+    const QPlan pl = q_plan(a.B, a.Tq, a.Tk, a.Hq, a.Hkv, DP, TILE);
+    a.packed = pl.packed;
+    a.splits = pl.splits;
+    a.split_rows = pl.split_rows;
+    if (pl.rs == 1) hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, 1, 1, 1>), dim3((unsigned)(pl.blocks * pl.splits)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, 1, WIDE, 1>), dim3((unsigned)(pl.blocks * pl.splits)), dim3(256), 0, s, a);
+    if (pl.splits > 1) {
+        const long long items = (long long)a.B * a.Hq * a.Tq * (a.D / 4);
+        hipLaunchKernelGGL(attn_lse_join_kernel<DT>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, a);
+    }
 }
 template <int DT>
 void launch_fwd(const Args& a, hipStream_t s) {
@@ -164,6 +232,10 @@ bool dp_attn_lse_tensor(const char* fn, const char* name, const void* ptr, const
     }
     const int n[3] = {B, Tn, H};
     for (int i = 0; i < 3; ++i) {
+        if (i == 1 && st[i] * es > 1 << 24) {
+            dp_set_error("%s: %s: tokens lie more than 2^24 bytes apart (%lld elements)", fn, name, st[i]);
+            return false;
+        }
         if (st[i] < 0 || (st[i] * es) % 16 != 0 || st[i] > (1LL << 40) || (written && n[i] > 1 && st[i] == 0)) {
             dp_set_error("%s: %s strides must be multiples of 16 bytes, of a written tensor also positive (got %lld elements at position %d)", fn, name, st[i], i);
             return false;
@@ -190,20 +262,34 @@ int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void*
     a->q_lens = q_lens;
     a->kv_lens = kv_lens;
     a->B = B; a->Tq = Tq; a->Tk = Tk; a->Hq = Hq; a->Hkv = Hkv; a->D = D;
-    a->Tqp = (Tq + 63) / 64 * 64;
+    a->Tqp = (Tq + 127) / 128 * 128;
+    a->splits = 1;
+    a->split_rows = 1 << 30;
     a->scale = scale;
     a->causal = causal != 0;
     a->xcd_map = dp_tune(DP_T_XCD_MAP) != 0;
     return 0;
 }
 
+extern "C" long long dp_attention_lse_workspace(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D) {
+    if (dtype < 0 || dtype > 2 || B <= 0 || Tq <= 0 || Tk <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return 0;
+    const al::QPlan pl = al::q_plan(B, Tq, Tk, Hq, Hkv, al::padded_dim(D), dtype == 0 ? 16 : 32);
+    return pl.splits > 1 ? (long long)pl.splits * B * Hq * Tq * (D + 1) * 4 : 0;
+}
+
 extern "C" int dp_attention_lse(const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq, int Hkv,
-                                int D, const int* q_lens, const int* kv_lens, float scale, int causal, void* out, float* lse, void* stream) {
+                                int D, const int* q_lens, const int* kv_lens, float scale, int causal, void* out, float* lse, void* work,
+                                long long work_bytes, void* stream) {
+    const char* fn = "dp_attention_lse";
     al::Args a{};
-    if (int rc = dp_attn_lse_common("dp_attention_lse", q, k, v, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, &a)) return rc;
-    DP_REQUIRE(lse, "dp_attention_lse: lse missing");
-    if (!dp_attn_lse_tensor("dp_attention_lse", "out", out, strides + 9, dtype == 0 ? 4 : 2, B, Tq, Hq, true, &a.w0)) return 1;
+    if (int rc = dp_attn_lse_common(fn, q, k, v, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, &a)) return rc;
+    DP_REQUIRE(lse, "%s: lse missing", fn);
+    if (!dp_attn_lse_tensor(fn, "out", out, strides + 9, dtype == 0 ? 4 : 2, B, Tq, Hq, true, &a.w0)) return 1;
+    const long long need = dp_attention_lse_workspace(dtype, B, Tq, Tk, Hq, Hkv, D);
+    DP_REQUIRE(need == 0 || (work && dp_aligned16(work) && work_bytes >= need), "%s: workspace of %lld bytes needed (got %lld)", fn, need, work_bytes);
     a.lse = lse;
+    a.part0 = static_cast<float*>(work);
+    a.part_lse = need ? a.part0 + need / 4 / (D + 1) * D : nullptr;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == 0) launch_fwd<0>(a, s);
     else if (dtype == 1) launch_fwd<1>(a, s);

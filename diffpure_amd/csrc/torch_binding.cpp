@@ -575,8 +575,11 @@ std::tuple<Tensor, Tensor> attention_lse(const Tensor& q, const Tensor& k, const
     c10::DeviceGuard guard(q.device());
     Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
     head_strides(out, "out", q, q.sizes(), st + 9);
+    const long long bytes = dp_attention_lse_workspace(n.code, n.b, n.tq, n.tk, n.hq, n.hkv, n.d);
+    Tensor work;
+    if (bytes) work = at::empty({bytes / 4}, q.options().dtype(at::kFloat));
     DP_CALL(dp_attention_lse(q.data_ptr(), k.data_ptr(), v.data_ptr(), st, n.code, n.b, n.tq, n.tk, n.hq, n.hkv, n.d, ql, kl, n.scale, causal, out.data_ptr(),
-                             lse.data_ptr<float>(), cur_stream(q)));
+                             lse.data_ptr<float>(), bytes ? work.data_ptr() : nullptr, bytes, cur_stream(q)));
     return {out, lse};
 }
 std::tuple<Tensor, Tensor, Tensor> attention_lse_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse,
@@ -594,7 +597,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_lse_bwd(const Tensor& dout, const T
     head_strides(dq, "dq", q, q.sizes(), st + 15);
     head_strides(dk, "dk", q, k.sizes(), st + 18);
     head_strides(dv, "dv", q, k.sizes(), st + 21);
-    const long long bytes = dp_attention_lse_bwd_workspace(n.b, n.tq, n.hq);
+    const long long bytes = dp_attention_lse_bwd_workspace(n.code, n.b, n.tq, n.tk, n.hq, n.hkv, n.d);
     Tensor work = at::empty({bytes / 4}, q.options().dtype(at::kFloat));
     DP_CALL(dp_attention_lse_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(), st, n.code, n.b, n.tq, n.tk, n.hq, n.hkv,
                                  n.d, ql, kl, n.scale, causal, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), bytes, cur_stream(q)));

@@ -1110,8 +1110,10 @@ def attention_lse(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
     with torch.cuda.device(q.device):
         out = torch.empty((b, tq, hq, d), device=q.device, dtype=q.dtype)
         lse = torch.empty((b, hq, tq), device=q.device, dtype=torch.float32)
-        st = (ctypes.c_longlong * 12)(*st, *out.stride()[:3])
-        _lib.call("dp_attention_lse", _ptr(q), _ptr(k), _ptr(v), ctypes.addressof(st), *args, int(bool(causal)), _ptr(out), _ptr(lse), _stream())
+        st = (ctypes.c_longlong * 12)(*st, *_heads(out, "attention_lse.out"))
+        nbytes = _lib.load().dp_attention_lse_workspace(*args[:7])
+        work = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32) if nbytes else None
+        _lib.call("dp_attention_lse", _ptr(q), _ptr(k), _ptr(v), ctypes.addressof(st), *args, int(bool(causal)), _ptr(out), _ptr(lse), _ptr(work), nbytes, _stream())
     return out, lse
 
 
@@ -1131,7 +1133,7 @@ def attention_lse_bwd(dout, q, k, v, out, lse, scale=None, causal=False, q_lens=
         for t, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
             st += _heads(t, f"attention_lse_bwd.{name}", q, like.shape)
         st = (ctypes.c_longlong * 24)(*st)
-        nbytes = _lib.load().dp_attention_lse_bwd_workspace(b, tq, hq)
+        nbytes = _lib.load().dp_attention_lse_bwd_workspace(*args[:7])
         work = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32)
         _lib.call("dp_attention_lse_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), ctypes.addressof(st), *args, int(bool(causal)),
                   _ptr(dq), _ptr(dk), _ptr(dv), _ptr(work), nbytes, _stream())

@@ -419,13 +419,15 @@ int dp_resize_affine_bwd(const float* dy, int B, int C, int Ho, int Wo, int out_
  *   causal != 0: row i of a sample sees keys 0 .. i + (keys - rows) of it (the last row sees every key).  Inside the lengths values must be finite for the mask to
  *     hide them.  A row that sees no key has out 0, lse -inf, and contributes no gradient.
  *   scale: finite, not 0.
- *   work of the backward pass: dp_attention_lse_bwd_workspace(B, Tq, Hq) bytes, 16-byte aligned, free again when the call's work on `stream` is
- *     done.  The outputs may not overlap any input.  Results do not depend on the order in which workgroups run (no atomics).
+ *   work: dp_attention_lse_workspace / dp_attention_lse_bwd_workspace bytes, 16-byte aligned, free again when the call's work on `stream` is done (the
+ *     forward pass needs none - 0 - where the queries fill the chip).  The outputs may not overlap any input.  Tokens of a tensor lie at most 2^24
+ *     bytes apart.  Results do not depend on the order in which workgroups run (no atomics).
  * The reference has no counterpart that keeps the statistics (QKVAttentionLegacy.forward, guided_diffusion/unet.py:345-362, materialises the weights and
  * autograd keeps or checkpoints them). */
 int dp_attention_lse(const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
-                     const int* q_lens, const int* kv_lens, float scale, int causal, void* out, float* lse, void* stream);
-long long dp_attention_lse_bwd_workspace(int B, int Tq, int Hq);
+                     const int* q_lens, const int* kv_lens, float scale, int causal, void* out, float* lse, void* work, long long work_bytes, void* stream);
+long long dp_attention_lse_workspace(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D);
+long long dp_attention_lse_bwd_workspace(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D);
 int dp_attention_lse_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides, int dtype,
                          int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, void* dq, void* dk,
                          void* dv, void* work, long long work_bytes, void* stream);

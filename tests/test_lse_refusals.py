@@ -12,9 +12,9 @@ def lib():
 PTR = 1 << 20          # never read: each call is refused
 
 
-def attn_fwd(q=PTR, k=PTR, v=PTR, out=PTR, lse=PTR, strides=None, dtype=1, b=2, tq=8, tk=8, hq=2, hkv=2, d=16, scale=0.25, strides_null=False):
+def attn_fwd(q=PTR, k=PTR, v=PTR, out=PTR, lse=PTR, strides=None, dtype=1, b=2, tq=8, tk=8, hq=2, hkv=2, d=16, scale=0.25, strides_null=False, work=None, nbytes=0):
     st = (C.c_longlong * 12)(*(strides or [h * t * d if i == 0 else (h * d if i == 1 else d) for h, t in ((hq, tq), (hkv, tk), (hkv, tk), (hq, tq)) for i in range(3)]))
-    return lib().dp_attention_lse(q, k, v, None if strides_null else C.addressof(st), dtype, b, tq, tk, hq, hkv, d, None, None, scale, 0, out, lse, None)
+    return lib().dp_attention_lse(q, k, v, None if strides_null else C.addressof(st), dtype, b, tq, tk, hq, hkv, d, None, None, scale, 0, out, lse, work, nbytes, None)
 
 
 @pytest.mark.parametrize("kw,what", [
@@ -23,7 +23,8 @@ def attn_fwd(q=PTR, k=PTR, v=PTR, out=PTR, lse=PTR, strides=None, dtype=1, b=2, 
     (dict(hq=3), b"multiple"), (dict(d=12), b"multiple of 8"), (dict(d=264), b"multiple of 8"), (dict(d=0), b"multiple of 8"), (dict(scale=0.0), b"scale"),
     (dict(scale=float("inf")), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(tq=(1 << 30) + 1), b"tokens"), (dict(b=1 << 20, hq=1 << 12, hkv=1 << 12), b"too many"),
     (dict(strides=[256, 32, 16] * 3 + [0, 32, 16]), b"also positive"), (dict(strides=[256, 32, 12] + [256, 32, 16] * 3), b"multiples"),
-    (dict(strides=[-256, 32, 16] + [256, 32, 16] * 3), b"multiples"),
+    (dict(strides=[-256, 32, 16] + [256, 32, 16] * 3), b"multiples"), (dict(strides=[256, 1 << 24, 16] + [256, 32, 16] * 3), b"apart"),
+    (dict(b=1, tq=1, tk=8000, hq=1, hkv=1), b"workspace"), (dict(b=1, tq=1, tk=8000, hq=1, hkv=1, work=PTR, nbytes=16), b"workspace"),
 ])
 def test_attention_lse_refuses(kw, what):
     assert attn_fwd(**kw) != 0
@@ -46,10 +47,13 @@ def test_attention_lse_bwd_refuses(kw, what):
 
 
 def test_attention_workspace_sizes():
-    ws = lib().dp_attention_lse_bwd_workspace
-    assert ws(0, 4, 4) == 0 and ws(1, 0, 4) == 0 and ws(1, 4, -1) == 0
-    assert ws(2, 65, 3) >= 2 * 2 * 3 * 128 * 4
-    assert ws(64, 1 << 20, 64) >= 2 * 64 * 64 * (1 << 20) * 4          # beyond 32 bits
+    fwd, bwd = lib().dp_attention_lse_workspace, lib().dp_attention_lse_bwd_workspace
+    for ws in (fwd, bwd):
+        assert ws(1, 0, 4, 4, 1, 1, 64) == 0 and ws(1, 1, 0, 4, 1, 1, 64) == 0 and ws(1, 1, 4, 4, 3, 2, 64) == 0 and ws(3, 1, 4, 4, 1, 1, 64) == 0 and ws(1, 1, 4, 4, 1, 1, 300) == 0
+    assert fwd(1, 64, 1024, 1024, 8, 8, 64) == 0                       # the queries fill the chip
+    assert fwd(2, 1, 1, 50000, 4, 1, 128) > 4 * 4 * 129                # a few rows over a long axis: partial results
+    assert bwd(1, 2, 65, 65, 3, 3, 64) >= 2 * 2 * 3 * 128 * 4
+    assert bwd(1, 64, 1 << 20, 8, 64, 64, 64) >= 2 * 64 * 64 * (1 << 20) * 4          # beyond 32 bits
 
 
 @pytest.mark.parametrize("kw,what", [
