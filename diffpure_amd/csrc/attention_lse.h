@@ -285,7 +285,18 @@ struct Args {
     int splits, split_rows;       // the streamed rows are cut into `splits` ranges of split_rows
     float scale;
     int causal, xcd_map;
+    int stripes;                  // causal: see block_of
 };
+
+// Block i of the nblk blocks of one head, longest first where a causal mask makes their work differ.  Contiguous ranges of blocks go to one XCD, so the
+// blocks of a head are dealt into `stripes` interleaved runs (as many as make every XCD's share a whole number of runs): each XCD gets long and short ones.
+__device__ __forceinline__ int block_of(const Args& p, int i, int nblk, bool longest_last) {
+    if (!p.causal) return i;
+    const int q = nblk / p.stripes, r = nblk - q * p.stripes, cut = r * (q + 1);
+    const int run = i < cut ? i / (q + 1) : r + (i - cut) / q, at = i < cut ? i % (q + 1) : (i - cut) % q;
+    const int blk = at * p.stripes + run;
+    return longest_last ? nblk - 1 - blk : blk;
+}
 
 // The kept queries of a workgroup.  Not packed: z = one query head, column = token.  Packed: z = one key head, column = head of the group * Tq + token.
 struct Kept {
@@ -311,6 +322,15 @@ namespace al {
 
 inline int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
 
+inline int stripes_of(long long heads) {
+    int s = 8;
+    while (s > 1 && heads % 2 == 0) {
+        heads /= 2;
+        s /= 2;
+    }
+    return s;
+}
+
 // How a launch that keeps queries (forward, dQ) covers the chip of 256 CUs.
 //   packed: heads that share their keys are columns of one block where all their queries fit two tiles (a key is then read once per group).
 //   rs:     waves of a workgroup that share one tile of columns and divide the streamed rows (1: every wave has its own columns).  Sharing makes
@@ -321,7 +341,7 @@ struct QPlan {
     long long blocks;
 };
 inline QPlan q_plan(int B, int Tq, int Tk, int Hq, int Hkv, int DP, int tile) {
-    QPlan pl;
+    QPlan pl;                     // (a block has 4 tiles of columns, or 4 / rs)
     const int group = Hq / Hkv;
     pl.packed = group > 1 && (long long)group * Tq <= 2 * tile;
     const long long heads = (long long)B * (pl.packed ? Hkv : Hq), cols = pl.packed ? (long long)group * Tq : Tq;
@@ -335,7 +355,8 @@ inline QPlan q_plan(int B, int Tq, int Tk, int Hq, int Hkv, int DP, int tile) {
     pl.splits = 1;
     const int stage = pl.rs * tile;
     if (pl.blocks < 256) {
-        const long long want = (512 + pl.blocks - 1) / pl.blocks, most = Tk / (4 * stage);
+        // one round of workgroups: the stages of two take 2 * 4 * tile rows of 2 * DP elements each, 160 KB hold two workgroups up to 64 channels
+        const long long fill = DP <= 64 ? 512 : 256, want = fill / pl.blocks, most = Tk / (4 * stage);
         pl.splits = (int)(want < most ? want : most);
         if (pl.splits < 1) pl.splits = 1;
         if (pl.splits > 128) pl.splits = 128;
@@ -348,34 +369,34 @@ inline QPlan q_plan(int B, int Tq, int Tk, int Hq, int Hkv, int DP, int tile) {
 
 // The same for the launch that keeps keys (dK, dV).  Its partial sums are as large as 2 * splits results, so it is split for causal launches (whose
 // blocks differ in length) and for those that would leave CUs without a workgroup.
+// Above 64 channels the two gradients are formed by different workgroups (each recomputes the scores): a wave that holds both has 64 or 128 accumulators
+// more and leaves no room for a second wave on its SIMD.
+constexpr bool two_roles(int DP) { return DP > 64; }
+
 struct KPlan {
-    int rs, splits, split_rows;
+    int rs, splits;
     long long blocks;
 };
-inline KPlan k_plan(int B, int Tq, int Tk, int Hq, int Hkv, int D, int DP, int tile, bool f32, int causal) {
-    (void)D;
-    (void)Hq;
+inline KPlan k_plan(int B, int Tq, int Tk, int Hkv, int DP, int tile, bool f32, int causal) {
     KPlan pl;
     const long long heads = (long long)B * Hkv;
+    const int roles = two_roles(DP) ? 2 : 1;
     pl.rs = 1;
     pl.blocks = heads * ((Tk + 4LL * tile - 1) / (4 * tile));
-    if (pl.blocks < 256) {
+    if (pl.blocks * roles < 256) {
         pl.rs = DP > 128 ? 2 : 4;
         const int wide = tile * 4 / pl.rs;
         pl.blocks = heads * ((Tk + wide - 1) / wide);
     }
     const int stage = pl.rs > 1 ? pl.rs * tile : (f32 ? 2 : 1) * tile;
     pl.splits = 1;
-    const long long enough = causal ? 1024 : 256;
-    if (pl.blocks < enough) {
-        const long long want = ((causal ? 1024 : 512) + pl.blocks - 1) / pl.blocks, most = Tq / (4 * stage);
+    const long long fill = causal ? 1024 : 512;
+    if (pl.blocks * roles < (causal ? 1024 : 256)) {
+        const long long want = (fill + pl.blocks * roles - 1) / (pl.blocks * roles), most = Tq / (4 * stage);
         pl.splits = (int)(want < most ? want : most);
         if (pl.splits < 1) pl.splits = 1;
         if (pl.splits > 64) pl.splits = 64;
     }
-    const int stages = (Tq + stage - 1) / stage;
-    pl.split_rows = (stages + pl.splits - 1) / pl.splits * stage;
-    pl.splits = (Tq + pl.split_rows - 1) / pl.split_rows;
     return pl;
 }
 

@@ -20,7 +20,8 @@ __global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_fwd_kernel(Args p) {
     const int rw = wave % RS, cl = lane & (T::TILE - 1), g = lane / T::TILE;
     const int bid0 = logical_block(p.xcd_map), split = bid0 % p.splits, bid = bid0 / p.splits;
     const int cols0 = p.packed ? p.Hq / p.Hkv * p.Tq : p.Tq, nblk = (cols0 + COLS - 1) / COLS;
-    const int z = bid / nblk, blk = p.causal ? nblk - 1 - (bid - z * nblk) : bid - z * nblk;     // causal: the long blocks first
+    const int z = bid / nblk, blk = block_of(p, bid - z * nblk, nblk, true);
+    if (z >= p.B * (p.packed ? p.Hkv : p.Hq)) return;
     const Kept kept(p, z);
     const int b = kept.b;
     const int n = clamp_len(p.q_lens, b, p.Tq), m = clamp_len(p.kv_lens, b, p.Tk), off = m - n;
@@ -184,14 +185,32 @@ __global__ __launch_bounds__(256) void attn_lse_join_kernel(Args p) {
     const Kept kept(p, z);
     int h, t;
     kept.col(p, (int)(kr - (long long)z * cols), h, t);
+    // eight loads under way at a time (ranges behind the last one repeat it with weight 0)
     float top = -INFINITY, sum = 0.f;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[s * rows + kr]);
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {
+        float l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l[i] = p.part_lse[min(s0 + i, p.splits - 1) * rows + kr];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, l[i]);
+    }
     f32x4 v = {};
     if (top > -INFINITY) {
-        for (int s = 0; s < p.splits; ++s) {
-            const float w = __builtin_amdgcn_exp2f((p.part_lse[s * rows + kr] - top) * LOG2E);
-            sum += w;
-            v += w * *reinterpret_cast<const f32x4*>(p.part0 + (s * rows + kr) * p.D + d);
+        for (int s0 = 0; s0 < p.splits; s0 += 8) {
+            float l[8];
+            f32x4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const long long at = min(s0 + i, p.splits - 1) * rows + kr;
+                l[i] = p.part_lse[at];
+                x[i] = *reinterpret_cast<const f32x4*>(p.part0 + at * p.D + d);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = s0 + i < p.splits ? __builtin_amdgcn_exp2f((l[i] - top) * LOG2E) : 0.f;
+                sum += w;
+                v += w * x[i];
+            }
         }
         v *= 1.f / sum;
     }
@@ -206,6 +225,7 @@ void launch_fwd(Args a, hipStream_t s) {
     a.packed = pl.packed;
     a.splits = pl.splits;
     a.split_rows = pl.split_rows;
+    a.stripes = stripes_of((long long)a.B * (pl.packed ? a.Hkv : a.Hq));
     if (pl.rs == 1) hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, 1, 1, 1>), dim3((unsigned)(pl.blocks * pl.splits)), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, 1, WIDE, 1>), dim3((unsigned)(pl.blocks * pl.splits)), dim3(256), 0, s, a);
     if (pl.splits > 1) {
@@ -253,7 +273,8 @@ int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void*
     DP_REQUIRE(Hq % Hkv == 0, "%s: %d query heads are not a multiple of %d key heads", fn, Hq, Hkv);
     DP_REQUIRE(D > 0 && D % 8 == 0 && D <= 256, "%s: the head dimension must be a multiple of 8 up to 256 (got %d)", fn, D);
     DP_REQUIRE(Tq <= (1 << 30) && Tk <= (1 << 30), "%s: at most 2^30 tokens (got %d, %d)", fn, Tq, Tk);
-    DP_REQUIRE((long long)B * Hq * ((Tq + 63) / 64) < (1LL << 31) && (long long)B * Hkv * ((Tk + 63) / 64) < (1LL << 31), "%s: too many blocks", fn);
+    const int cols = dtype == 0 ? 64 : 128;       // a grid has fewer than 2^32 threads; the launch that keeps keys has up to two workgroups of 256 per block
+    DP_REQUIRE((long long)B * Hq * ((Tq + cols - 1) / cols) < (1LL << 23) && (long long)B * Hkv * ((Tk + cols - 1) / cols) < (1LL << 23), "%s: too many blocks", fn);
     DP_REQUIRE(scale != 0.f && scale - scale == 0.f, "%s: the scale must be finite and not zero", fn);
     const int es = dtype == 0 ? 4 : 2;
     if (!dp_attn_lse_tensor(fn, "q", q, strides, es, B, Tq, Hq, false, &a->q) || !dp_attn_lse_tensor(fn, "k", k, strides + 3, es, B, Tk, Hkv, false, &a->k) ||

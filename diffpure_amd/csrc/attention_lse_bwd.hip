@@ -14,7 +14,7 @@ using namespace al;
 
 // dQ.  Workgroups, stages and RS as in the forward kernel.
 template <int DT, int DP, int CW, int RS, int RT>
-__global__ __launch_bounds__(256) AL_WAVES(DP <= 128 ? 2 : 1) void attn_lse_dq_kernel(Args p) {
+__global__ __launch_bounds__(256) AL_WAVES(DT && DP == 64 && RS == 1 ? 3 : DP <= 128 ? 2 : 1) void attn_lse_dq_kernel(Args p) {
     using T = Tr<DT>;
     constexpr int NW = 4, BM = RS * RT * T::TILE, RB = DP * T::ES, KS = DP / 16, ND = DP / T::TILE, NKK = T::TILE / 16, COLS = NW / RS * CW * T::TILE;
     using St = Stream<RB, T::ES, BM, NW>;
@@ -23,7 +23,8 @@ __global__ __launch_bounds__(256) AL_WAVES(DP <= 128 ? 2 : 1) void attn_lse_dq_k
     const int rw = wave % RS, cl = lane & (T::TILE - 1), g = lane / T::TILE;
     const int bid0 = logical_block(p.xcd_map), split = bid0 % p.splits, bid = bid0 / p.splits;
     const int cols0 = p.packed ? p.Hq / p.Hkv * p.Tq : p.Tq, nblk = (cols0 + COLS - 1) / COLS;
-    const int z = bid / nblk, blk = p.causal ? nblk - 1 - (bid - z * nblk) : bid - z * nblk;
+    const int z = bid / nblk, blk = block_of(p, bid - z * nblk, nblk, true);
+    if (z >= p.B * (p.packed ? p.Hkv : p.Hq)) return;
     const Kept kept(p, z);
     const int b = kept.b;
     const int n = clamp_len(p.q_lens, b, p.Tq), m = clamp_len(p.kv_lens, b, p.Tk), off = m - n;
@@ -164,59 +165,80 @@ __global__ __launch_bounds__(256) AL_WAVES(DP <= 128 ? 2 : 1) void attn_lse_dq_k
     }
 }
 
-// dK and dV: keys are kept, the queries of every head of the group stream by, one head after the other.
-template <int DT, int DP, int CW, int RS, int RT>
-__global__ __launch_bounds__(256) AL_WAVES(DP <= (DT == 0 ? 128 : 64) ? 2 : 1) void attn_lse_dkv_kernel(Args p) {
+// dK and dV: keys are kept, the queries of every head of the group stream by, one head after the other.  WHAT: 1 dK, 2 dV, 3 both.
+template <int DT, int DP, int CW, int RS, int RT> struct Dkv {
+    static constexpr int NW = 4, BM = RS * RT * Tr<DT>::TILE, RB = DP * Tr<DT>::ES;
+    using St = Stream<RB, Tr<DT>::ES, BM, NW>;
+    struct Shared {
+        char stage[2 * St::STAGE];
+        float rows[2][2][BM];             // stage: log-sum-exp, -delta of the streamed queries
+    };
+};
+template <int DT, int DP, int CW, int RS, int RT, int WHAT>
+__device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<DT, DP, CW, RS, RT>::Shared& sh) {
     using T = Tr<DT>;
-    constexpr int NW = 4, BM = RS * RT * T::TILE, RB = DP * T::ES, KS = DP / 16, ND = DP / T::TILE, NKK = T::TILE / 16, COLS = NW / RS * CW * T::TILE;
-    using St = Stream<RB, T::ES, BM, NW>;
+    using K = Dkv<DT, DP, CW, RS, RT>;
+    using St = typename K::St;
+    constexpr int NW = K::NW, BM = K::BM, RB = K::RB, KS = DP / 16, ND = DP / T::TILE, NKK = T::TILE / 16, COLS = NW / RS * CW * T::TILE;
+    constexpr bool DK = WHAT & 1, DV = WHAT & 2;
     static_assert(BM % 32 == 0 && BM <= 128, "whole waves copy the rows' statistics, of which a multiple of 128 exist");
-    __shared__ __attribute__((aligned(1024))) char smem[2 * St::STAGE];
-    __shared__ __attribute__((aligned(16))) float rows[2][2][BM];       // stage: log-sum-exp, -delta of the streamed queries
+    char* smem = sh.stage;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = wave % RS, cl = lane & (T::TILE - 1), g = lane / T::TILE;
-    const int bid0 = logical_block(p.xcd_map), split = bid0 % p.splits, bid = bid0 / p.splits;
+    const int split = bid0 % p.splits, bid = bid0 / p.splits;
     const int nblk = (p.Tk + COLS - 1) / COLS, group = p.Hq / p.Hkv;
-    const int z = bid / nblk, blk = bid - z * nblk;                    // causal: the first blocks are the long ones
+    const int z = bid / nblk, blk = block_of(p, bid - z * nblk, nblk, false);
+    if (z >= p.B * p.Hkv) return;
     const int b = z / p.Hkv, hk = z - b * p.Hkv;
     const int n = clamp_len(p.q_lens, b, p.Tq), m = clamp_len(p.kv_lens, b, p.Tk), off = m - n;
     const int c0 = blk * COLS, wc0 = c0 + wave / RS * CW * T::TILE;
     const int row_slots = p.D * T::ES / 16;
     const float c = p.scale * LOG2E;
 
-    typename T::Frag kf[CW][KS], vf[CW][KS];
-    typename T::Acc dk[CW][ND], dv[CW][ND];
+    typename T::Frag kf[CW][KS], vf[CW][DK ? KS : 1];
+    typename T::Acc dk[CW][DK ? ND : 1], dv[CW][DV ? ND : 1];
 #pragma unroll
     for (int cw = 0; cw < CW; ++cw) {
         const int col = wc0 + cw * T::TILE + cl, row = col < m ? col : (m > 0 ? m - 1 : 0);
         ld_kept<DT, KS>(kf[cw], p.k.p + b * p.k.b + hk * p.k.h + row * p.k.t, row_slots, g);
-        ld_kept<DT, KS>(vf[cw], p.v.p + b * p.v.b + hk * p.v.h + row * p.v.t, row_slots, g);
+        if constexpr (DK) ld_kept<DT, KS>(vf[cw], p.v.p + b * p.v.b + hk * p.v.h + row * p.v.t, row_slots, g);
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt) dk[cw][dt] = dv[cw][dt] = typename T::Acc{};
+        for (int dt = 0; dt < ND; ++dt) {
+            if constexpr (DK) dk[cw][dt] = typename T::Acc{};
+            if constexpr (DV) dv[cw][dt] = typename T::Acc{};
+        }
     }
 
-    // streamed rows of each head: [begin, open) through the causal mask, [open, end) see every column
-    int begin = split * p.split_rows, end = c0 < m ? min(n, begin + p.split_rows) : 0, open = begin;
-    if (p.causal) {
-        begin = max(begin, (c0 - off) / BM * BM);                      // the first query that sees a key of this workgroup (rounded down)
-        open = begin + (max(min(end, c0 + COLS - 1 - off) - begin, 0) + BM - 1) / BM * BM;
+    // Streamed rows of each head: [begin, open) through the causal mask, [open, end) see every column.  A split launch cuts a block's own rows into equal
+    // ranges: with the longest blocks first, two ranges each, the long and the short ones that meet on a CU add up alike.
+    int begin = 0, end = c0 < m ? n : 0, open = 0;
+    if (p.causal) begin = max(0, (c0 - off) / BM * BM);                // the first query that sees a key of this workgroup (rounded down)
+    if (p.splits > 1) {
+        const int range = ((max(end - begin, 0) + p.splits - 1) / p.splits + BM - 1) / BM * BM;
+        begin += split * range;
+        end = min(end, begin + range);
     }
+    if (p.causal) open = begin + (max(min(end, c0 + COLS - 1 - off) - begin, 0) + BM - 1) / BM * BM;
+    else open = begin;
     St st;
     st.init(p.q.p + b * p.q.b + hk * group * p.q.h, p.q.t, p.dout.p + b * p.dout.b + hk * group * p.dout.h, p.dout.t, row_slots, wave, lane);
     // lane t < 2 BM of the workgroup copies one value of a tile: log-sum-exp (t < BM) or -delta of query t % BM
     const float* mine = p.rows + ((long long)b * p.Hq + hk * group) * p.Tqp + (tid < BM ? tid : (long long)p.B * p.Hq * p.Tqp + tid - BM);
     auto issue = [&](int stage, int head, int r0) {
         st.issue(smem + stage * St::STAGE, r0, n, head * p.q.h, head * p.dout.h);
-        if (wave * 64 < 2 * BM) AL_GLDS(mine + (long long)head * p.Tqp + r0, reinterpret_cast<char*>(&rows[stage][0][0]) + wave * 256, 4);
+        if (wave * 64 < 2 * BM) AL_GLDS(mine + (long long)head * p.Tqp + r0, reinterpret_cast<char*>(&sh.rows[stage][0][0]) + wave * 256, 4);
     };
+    // Rows are taken from the last one down: a causal mask lets the blocks of a head begin at different rows but end at the same one, and the blocks that run
+    // at a time share what they stream (in L2) only while they stand at the same row.
+    const int last = begin + (end - begin - 1) / BM * BM;
     int cur = 0;
     auto body = [&](int head, int r0, auto masked) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        const bool wrap = r0 + BM >= end;
-        if (!wrap || head + 1 < group) issue(cur ^ 1, wrap ? head + 1 : head, wrap ? begin : r0 + BM);
+        const bool wrap = r0 == begin;
+        if (!wrap || head + 1 < group) issue(cur ^ 1, wrap ? head + 1 : head, wrap ? last : r0 - BM);
         const char* stage = smem + cur * St::STAGE;
-        const float(*rs)[BM] = rows[cur];
+        const float(*rs)[BM] = sh.rows[cur];
         cur ^= 1;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -226,7 +248,8 @@ __global__ __launch_bounds__(256) AL_WAVES(DP <= (DT == 0 ? 128 : 64) ? 2 : 1) v
 #pragma unroll
             for (int r = 0; r < T::NR; r += 4) {
                 const f32x4 x = *reinterpret_cast<const f32x4*>(&rs[0][rr + r * T::G + 4 * g]);
-                const f32x4 y = *reinterpret_cast<const f32x4*>(&rs[1][rr + r * T::G + 4 * g]);
+                f32x4 y = {};
+                if constexpr (DK) y = *reinterpret_cast<const f32x4*>(&rs[1][rr + r * T::G + 4 * g]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     l2[r + j] = x[j];
@@ -241,11 +264,13 @@ __global__ __launch_bounds__(256) AL_WAVES(DP <= (DT == 0 ? 128 : 64) ? 2 : 1) v
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const typename T::Frag aq = ld_row<DT, RB>(Qs, lane, ks), ad = ld_row<DT, RB>(Ds, lane, ks);
+                const typename T::Frag aq = ld_row<DT, RB>(Qs, lane, ks);
 #pragma unroll
-                for (int cw = 0; cw < CW; ++cw) {
-                    s[cw] = T::mma(aq, kf[cw][ks], s[cw]);
-                    ds[cw] = T::mma(ad, vf[cw][ks], ds[cw]);
+                for (int cw = 0; cw < CW; ++cw) s[cw] = T::mma(aq, kf[cw][ks], s[cw]);
+                if constexpr (DK) {
+                    const typename T::Frag ad = ld_row<DT, RB>(Ds, lane, ks);
+#pragma unroll
+                    for (int cw = 0; cw < CW; ++cw) ds[cw] = T::mma(ad, vf[cw][ks], ds[cw]);
                 }
             }
 #pragma unroll
@@ -269,16 +294,20 @@ __global__ __launch_bounds__(256) AL_WAVES(DP <= (DT == 0 ? 128 : 64) ? 2 : 1) v
                 typename T::Frag pf[CW], sf[CW];
 #pragma unroll
                 for (int cw = 0; cw < CW; ++cw) {
-                    pf[cw] = pack<DT>(s[cw], kk);
-                    sf[cw] = pack<DT>(ds[cw], kk);
+                    if constexpr (DV) pf[cw] = pack<DT>(s[cw], kk);
+                    if constexpr (DK) sf[cw] = pack<DT>(ds[cw], kk);
                 }
 #pragma unroll
                 for (int dt = 0; dt < ND; ++dt) {
-                    const typename T::Frag ad = ld_tr<DT, RB>(Ds, lane, kk, dt), aq = ld_tr<DT, RB>(Qs, lane, kk, dt);
+                    if constexpr (DV) {
+                        const typename T::Frag ad = ld_tr<DT, RB>(Ds, lane, kk, dt);
 #pragma unroll
-                    for (int cw = 0; cw < CW; ++cw) {
-                        dv[cw][dt] = T::mma(ad, pf[cw], dv[cw][dt]);
-                        dk[cw][dt] = T::mma(aq, sf[cw], dk[cw][dt]);
+                        for (int cw = 0; cw < CW; ++cw) dv[cw][dt] = T::mma(ad, pf[cw], dv[cw][dt]);
+                    }
+                    if constexpr (DK) {
+                        const typename T::Frag aq = ld_tr<DT, RB>(Qs, lane, kk, dt);
+#pragma unroll
+                        for (int cw = 0; cw < CW; ++cw) dk[cw][dt] = T::mma(aq, sf[cw], dk[cw][dt]);
                     }
                 }
             }
@@ -286,11 +315,11 @@ __global__ __launch_bounds__(256) AL_WAVES(DP <= (DT == 0 ? 128 : 64) ? 2 : 1) v
         settle();
     };
     if (begin < end) {
-        issue(0, 0, begin);
+        issue(0, 0, last);
         for (int head = 0; head < group; ++head) {
-            int r0 = begin;
-            for (; r0 < open; r0 += BM) body(head, r0, yes{});
-            for (; r0 < end; r0 += BM) body(head, r0, no{});
+            int r0 = last;
+            for (; r0 >= open; r0 -= BM) body(head, r0, no{});
+            for (; r0 >= begin; r0 -= BM) body(head, r0, yes{});
         }
     }
 
@@ -307,11 +336,25 @@ __global__ __launch_bounds__(256) AL_WAVES(DP <= (DT == 0 ? 128 : 64) ? 2 : 1) v
             if (p.splits > 1) *reinterpret_cast<f32x4*>(part + kr * p.D + d) = v;
             else st4<DT>(const_cast<char*>(w.p) + b * w.b + hk * w.h + col * w.t, d, v);
         };
-        if constexpr (RS > 1) __syncthreads();
-        join_units<DT, ND, RS>(dk[cw], p.scale * pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w0, p.part0, u, v); });
-        if constexpr (RS > 1) __syncthreads();
-        join_units<DT, ND, RS>(dv[cw], pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w1, p.part1, u, v); });
+        if constexpr (DK) {
+            if constexpr (RS > 1) __syncthreads();
+            join_units<DT, ND, RS>(dk[cw], p.scale * pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w0, p.part0, u, v); });
+        }
+        if constexpr (DV) {
+            if constexpr (RS > 1) __syncthreads();
+            join_units<DT, ND, RS>(dv[cw], pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w1, p.part1, u, v); });
+        }
     }
+}
+
+template <int DT, int DP, int CW, int RS, int RT>
+__global__ __launch_bounds__(256) AL_WAVES(DP > 128 ? 1 : DT && DP == 64 && RS == 1 ? 3 : 2) void attn_lse_dkv_kernel(Args p) {
+    __shared__ __attribute__((aligned(1024))) typename Dkv<DT, DP, CW, RS, RT>::Shared sh;
+    const int bid = logical_block(p.xcd_map);
+    if constexpr (two_roles(DP)) {
+        if (bid & 1) dkv_block<DT, DP, CW, RS, RT, 2>(p, bid >> 1, sh);
+        else dkv_block<DT, DP, CW, RS, RT, 1>(p, bid >> 1, sh);
+    } else dkv_block<DT, DP, CW, RS, RT, 3>(p, bid, sh);
 }
 
 // sums of the ranges of a split launch, in their order: part [split][rows][D] -> rows of a [B, T, H, D] tensor.  Packed as the kept queries are, or plain
@@ -349,6 +392,7 @@ void launch_bwd(const Args& a, const Ten& dq, const Ten& dk, const Ten& dv, hipS
     x.packed = pq.packed;
     x.splits = pq.splits;
     x.split_rows = pq.split_rows;
+    x.stripes = stripes_of((long long)a.B * (pq.packed ? a.Hkv : a.Hq));
     const dim3 gq((unsigned)(pq.blocks * pq.splits));
     if (pq.rs == 1) hipLaunchKernelGGL((attn_lse_dq_kernel<DT, DP, 1, 1, 1>), gq, wg, 0, s, x);
     else hipLaunchKernelGGL((attn_lse_dq_kernel<DT, DP, 1, WIDE, 1>), gq, wg, 0, s, x);
@@ -359,11 +403,11 @@ void launch_bwd(const Args& a, const Ten& dq, const Ten& dk, const Ten& dv, hipS
     x.w0 = dk;
     x.w1 = dv;
     x.packed = 0;
-    const KPlan pk = k_plan(a.B, a.Tq, a.Tk, a.Hq, a.Hkv, a.D, DP, TILE, DT == 0, a.causal);
+    const KPlan pk = k_plan(a.B, a.Tq, a.Tk, a.Hkv, DP, TILE, DT == 0, a.causal);
+    x.stripes = stripes_of((long long)a.B * a.Hkv);
     x.splits = pk.splits;
-    x.split_rows = pk.split_rows;
     x.part1 = x.part0 + (long long)pk.splits * a.B * a.Hkv * a.Tk * a.D;
-    const dim3 gk((unsigned)(pk.blocks * pk.splits));
+    const dim3 gk((unsigned)(pk.blocks * pk.splits * (two_roles(DP) ? 2 : 1)));
     if (pk.rs == 1) hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, 1, 1, RT>), gk, wg, 0, s, x);
     else hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, 1, WIDE, 1>), gk, wg, 0, s, x);
     if (pk.splits > 1) {
@@ -386,7 +430,7 @@ extern "C" long long dp_attention_lse_bwd_workspace(int dtype, int B, int Tq, in
     if (dtype < 0 || dtype > 2 || B <= 0 || Tq <= 0 || Tk <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return 0;
     const int tile = dtype == 0 ? 16 : 32, DP = al::padded_dim(D);
     const al::QPlan pq = al::q_plan(B, Tq, Tk, Hq, Hkv, DP, tile);
-    const al::KPlan pk = al::k_plan(B, Tq, Tk, Hq, Hkv, D, DP, tile, dtype == 0, 1), pk0 = al::k_plan(B, Tq, Tk, Hq, Hkv, D, DP, tile, dtype == 0, 0);
+    const al::KPlan pk = al::k_plan(B, Tq, Tk, Hkv, DP, tile, dtype == 0, 1), pk0 = al::k_plan(B, Tq, Tk, Hkv, DP, tile, dtype == 0, 0);
     const long long rows = 2LL * B * Hq * ((Tq + 127LL) / 128 * 128);
     const long long q = pq.splits > 1 ? (long long)pq.splits * B * Hq * Tq * D : 0;
     const int ks = pk.splits > pk0.splits ? pk.splits : pk0.splits;
