@@ -40,51 +40,83 @@ __device__ __forceinline__ void settle() {
 
 constexpr float LOG2E = 1.44269504088896341f;
 
-// DT: element type of q, k, v, out and the gradients (0 fp32, 1 fp16, 2 bf16).
-//   TILE columns / rows of a score tile, G lane groups of TILE lanes, NR accumulator registers per tile.
-//   Register r of lane l is row (r & 3) + 4 G (r >> 2) + 4 (l / TILE), column l % TILE.
+// DT: element type of q, k, v, out and the gradients, and the shape of a score tile
+//   0 fp32, 1 fp16, 2 bf16; 3, 4: fp16, bf16 with 16 columns (above 128 channels: half the registers for the kept operand and the accumulators)
+//   TILE columns of a tile, G lane groups of TILE lanes; an accumulator holds TILE rows in NR registers:
+//   register r of lane l is row (r & 3) + 4 G (r >> 2) + 4 (l / TILE), column l % TILE; a score tile is SUB of them, ROWS = SUB TILE rows.
+//   KSTEP channels per step of the first product, KROWS rows per step of the second.
 //   PSHIFT: the backward pass forms 2^PSHIFT P (an addend of the exponent, free) - see attention_lse_bwd.hip.
 template <int DT> struct Tr;
-template <> struct Tr<1> {
+struct Half {
     typedef _Float16 E;
     typedef f16x8 Frag;
     typedef f16x4 E4;
-    typedef f32x16 Acc;
-    static constexpr int TILE = 32, G = 2, NR = 16, ES = 2, PSHIFT = 6;
-    static __device__ __forceinline__ Acc mma(Frag a, Frag b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static constexpr int ES = 2, PSHIFT = 6;
 };
-template <> struct Tr<2> {
+struct Bf {
     typedef __bf16 E;
     typedef bf16x8 Frag;
     typedef bf16x4 E4;
+    static constexpr int ES = 2, PSHIFT = 0;
+};
+struct Wide {
     typedef f32x16 Acc;
-    static constexpr int TILE = 32, G = 2, NR = 16, ES = 2, PSHIFT = 0;
+    static constexpr int TILE = 32, G = 2, NR = 16, SUB = 1, ROWS = 32, KSTEP = 16, KROWS = 16;
+};
+struct Narrow {
+    typedef f32x4 Acc;
+    static constexpr int TILE = 16, G = 4, NR = 4, SUB = 2, ROWS = 32, KSTEP = 32, KROWS = 32;
+};
+template <> struct Tr<1> : Half, Wide {
+    static __device__ __forceinline__ Acc mma(Frag a, Frag b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Tr<2> : Bf, Wide {
     static __device__ __forceinline__ Acc mma(Frag a, Frag b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Tr<3> : Half, Narrow {
+    static __device__ __forceinline__ Acc mma(Frag a, Frag b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Tr<4> : Bf, Narrow {
+    static __device__ __forceinline__ Acc mma(Frag a, Frag b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Tr<0> {
     typedef float E;
     typedef f32x4 Frag;
     typedef f32x4 E4;
     typedef f32x4 Acc;
-    static constexpr int TILE = 16, G = 4, NR = 4, ES = 4, PSHIFT = 0;
+    static constexpr int TILE = 16, G = 4, NR = 4, SUB = 1, ROWS = 16, KSTEP = 16, KROWS = 16, ES = 4, PSHIFT = 0;
     static __device__ __forceinline__ Acc mma(Frag a, Frag b, Acc c) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
         return c;
     }
 };
+// the shape of a type at a (padded) head dimension
+constexpr int shape_of(int dtype, int DP) { return dtype && DP > 128 ? dtype + 2 : dtype; }
+constexpr int tile_of(int dtype, int DP) { return dtype == 0 || DP > 128 ? 16 : 32; }
 
-// registers 8 kk .. 8 kk + 7 (fp32: all four) of a score tile -> B operand of step kk of the second product
-template <int DT>
-__device__ __forceinline__ typename Tr<DT>::Frag pack(const typename Tr<DT>::Acc& p, int kk) {
-    if constexpr (DT == 0) return p;
-    else {
-        typename Tr<DT>::Frag f;
+// a score tile: [ROWS streamed rows] x [TILE kept columns]
+template <int DT> struct Score {
+    using T = Tr<DT>;
+    static constexpr int N = T::SUB * T::NR;
+    typename T::Acc a[T::SUB];
+    __device__ __forceinline__ float get(int r) const { return a[r / T::NR][r % T::NR]; }
+    __device__ __forceinline__ void set(int r, float v) { a[r / T::NR][r % T::NR] = v; }
+    __device__ __forceinline__ void fill(float v) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (typename Tr<DT>::E)p[kk * 8 + j];
-        return f;
+        for (int r = 0; r < N; ++r) set(r, v);
     }
-}
+    // -> B operand of step kk of the second product
+    __device__ __forceinline__ typename T::Frag pack(int kk) const {
+        if constexpr (DT == 0) return a[0];
+        else {
+            typename T::Frag f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = (typename T::E)get(kk * 8 + j);
+            return f;
+        }
+    }
+};
 
 // LDS image of a streamed tile: rows of RB bytes, the 16-byte slots of a row XOR-ed with bits of the row.  The 64 banks take 16 slots at a time, so
 //   - a row read (one slot of 16 consecutive rows) wants 16 different places for the rows, and
@@ -94,7 +126,7 @@ __device__ __forceinline__ typename Tr<DT>::Frag pack(const typename Tr<DT>::Acc
 template <int RB, int ES> struct Lds {
     static constexpr int SLOTS = RB / 16;
     static __device__ __forceinline__ int swz(int row) {
-        if constexpr (SLOTS % 16 == 0) return ES == 4 ? row & 15 : ((row & 3) << 2) | ((row >> 2) & 3);
+        if constexpr (SLOTS % 16 == 0) return ES == 4 ? row & 15 : ((row & 3) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1);
         else if constexpr (SLOTS % 8 == 0) return ES == 4 ? (row >> 1) & 7 : ((row & 2) << 1) | ((row >> 2) & 3);
         else return (row >> 2) & 3;
     }
@@ -108,7 +140,15 @@ __device__ __forceinline__ typename Tr<DT>::Frag ld_row(const char* tile, int la
     return *reinterpret_cast<const typename T::Frag*>(tile + Lds<RB, T::ES>::at(lane & (T::TILE - 1), ks * T::G + lane / T::TILE));
 }
 
-// A operand, transposed: row = d of block dt, k = the 16 streamed rows of step kk in the accumulator's order
+// the first product, one step: score += [streamed rows] x [kept columns]
+template <int DT, int RB>
+__device__ __forceinline__ void mma_rows(const char* tile, int lane, int ks, typename Tr<DT>::Frag kept, Score<DT>& s) {
+    using T = Tr<DT>;
+#pragma unroll
+    for (int i = 0; i < T::SUB; ++i) s.a[i] = T::mma(ld_row<DT, RB>(tile + i * T::TILE * RB, lane, ks), kept, s.a[i]);
+}
+
+// A operand, transposed: row = d of block dt, k = the KROWS streamed rows of step kk in the accumulator's order
 template <int DT, int RB>
 __device__ __forceinline__ typename Tr<DT>::Frag ld_tr(const char* tile, int lane, int kk, int dt) {
     using T = Tr<DT>;
@@ -119,10 +159,10 @@ __device__ __forceinline__ typename Tr<DT>::Frag ld_tr(const char* tile, int lan
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(tile + Lds<RB, T::ES>::at(4 * g + j, byte >> 4) + (byte & 12));
     } else {
-        const int i = lane & 15, byte = (dt * 32 + (lane & 16) + 4 * (i & 3)) * 2;
+        const int i = lane & 15, byte = (dt * T::TILE + (lane & (T::TILE - 16)) + 4 * (i & 3)) * 2;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const int row = kk * 16 + half * 8 + 4 * g + (i >> 2);
+            const int row = kk * 16 + half * 4 * T::G + 4 * g + (i >> 2);
             const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) s16x4*)(tile + Lds<RB, T::ES>::at(row, byte >> 4) + (byte & 8)));
             const typename T::E4 e = __builtin_bit_cast(typename T::E4, v);
@@ -263,7 +303,7 @@ __device__ __forceinline__ void join_units(const typename Tr<DT>::Acc (&acc)[ND]
     }
 }
 
-// row of the tile that register r holds (plus 4 g)
+// row of the tile that register r of a score holds (plus 4 g)
 template <int DT> __device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 4 * Tr<DT>::G * (r >> 2); }
 
 // [B, T, H, D] tensor: byte strides
@@ -340,9 +380,9 @@ struct QPlan {
     int packed, rs, splits, split_rows;
     long long blocks;
 };
-inline QPlan q_plan(int B, int Tq, int Tk, int Hq, int Hkv, int DP, int tile) {
-    QPlan pl;                     // (a block has 4 tiles of columns, or 4 / rs)
-    const int group = Hq / Hkv;
+inline QPlan q_plan(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int DP) {
+    QPlan pl;                     // a block has 4 / rs tiles of columns
+    const int group = Hq / Hkv, tile = tile_of(dtype, DP), srows = dtype == 0 ? 16 : 32;
     pl.packed = group > 1 && (long long)group * Tq <= 2 * tile;
     const long long heads = (long long)B * (pl.packed ? Hkv : Hq), cols = pl.packed ? (long long)group * Tq : Tq;
     pl.rs = 1;
@@ -353,7 +393,7 @@ inline QPlan q_plan(int B, int Tq, int Tk, int Hq, int Hkv, int DP, int tile) {
         pl.blocks = heads * ((cols + wide - 1) / wide);
     }
     pl.splits = 1;
-    const int stage = pl.rs * tile;
+    const int stage = pl.rs * srows;
     if (pl.blocks < 256) {
         // one round of workgroups: the stages of two take 2 * 4 * tile rows of 2 * DP elements each, 160 KB hold two workgroups up to 64 channels
         const long long fill = DP <= 64 ? 512 : 256, want = fill / pl.blocks, most = Tk / (4 * stage);
@@ -369,18 +409,18 @@ inline QPlan q_plan(int B, int Tq, int Tk, int Hq, int Hkv, int DP, int tile) {
 
 // The same for the launch that keeps keys (dK, dV).  Its partial sums are as large as 2 * splits results, so it is split for causal launches (whose
 // blocks differ in length) and for those that would leave CUs without a workgroup.
-// Above 64 channels the two gradients are formed by different workgroups (each recomputes the scores): a wave that holds both has 64 or 128 accumulators
-// more and leaves no room for a second wave on its SIMD.
-constexpr bool two_roles(int DP) { return DP > 64; }
+// Above 64 channels (tiles of 32 columns, fp32) the two gradients are formed by different workgroups, each of which recomputes the scores: a wave that
+// holds both has 64 accumulators more and leaves no room for a second wave on its SIMD (8191 causal, heads of 128: 1434 us together, 1160 us apart).
+constexpr bool two_roles(int dtype, int DP) { return DP > 64 && shape_of(dtype, DP) < 3; }
 
 struct KPlan {
     int rs, splits;
     long long blocks;
 };
-inline KPlan k_plan(int B, int Tq, int Tk, int Hkv, int DP, int tile, bool f32, int causal) {
+inline KPlan k_plan(int dtype, int B, int Tq, int Tk, int Hkv, int DP, int causal) {
     KPlan pl;
     const long long heads = (long long)B * Hkv;
-    const int roles = two_roles(DP) ? 2 : 1;
+    const int roles = two_roles(dtype, DP) ? 2 : 1, tile = tile_of(dtype, DP);
     pl.rs = 1;
     pl.blocks = heads * ((Tk + 4LL * tile - 1) / (4 * tile));
     if (pl.blocks * roles < 256) {
@@ -388,7 +428,7 @@ inline KPlan k_plan(int B, int Tq, int Tk, int Hkv, int DP, int tile, bool f32, 
         const int wide = tile * 4 / pl.rs;
         pl.blocks = heads * ((Tk + wide - 1) / wide);
     }
-    const int stage = pl.rs > 1 ? pl.rs * tile : (f32 ? 2 : 1) * tile;
+    const int stage = pl.rs * (dtype == 0 ? 16 : 32);
     pl.splits = 1;
     const long long fill = causal ? 1024 : 512;
     if (pl.blocks * roles < (causal ? 1024 : 256)) {

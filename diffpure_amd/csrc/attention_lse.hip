@@ -5,17 +5,17 @@
 namespace {
 using namespace al;
 
-// One workgroup = 4 waves; K and V tiles stream through LDS (double buffered).  RS = 1: every wave has its own CW tiles of query columns and sees every
+// One workgroup = 4 waves; K and V tiles stream through LDS (double buffered).  RS = 1: every wave has its own tile of query columns and sees every
 // streamed row.  RS > 1 (few columns): RS waves share their columns and take different rows of a stage; they join at the end.
 // The running maximum is only moved when a row's maximum has grown by more than 8 (in log2): until then the probabilities are taken
 // against the old one - at most 2^8, exact in every type's range - and neither sum nor output is rescaled.
-template <int DT, int DP, int CW, int RS, int RT>
+template <int DT, int DP, int RS>
 __global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_fwd_kernel(Args p) {
     using T = Tr<DT>;
-    constexpr int NW = 4, BM = RS * RT * T::TILE, RB = DP * T::ES, KS = DP / 16, ND = DP / T::TILE, NKK = T::TILE / 16, COLS = NW / RS * CW * T::TILE;
+    constexpr int NW = 4, BM = RS * T::ROWS, RB = DP * T::ES, KS = DP / T::KSTEP, ND = DP / T::TILE, NKK = T::ROWS / T::KROWS, COLS = NW / RS * T::TILE;
     using St = Stream<RB, T::ES, BM, NW>;
     __shared__ __attribute__((aligned(1024))) char smem[2 * St::STAGE];
-    __shared__ float ml[RS > 1 ? 2 : 1][NW][CW * T::TILE];
+    __shared__ float ml[RS > 1 ? 2 : 1][NW][T::TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rw = wave % RS, cl = lane & (T::TILE - 1), g = lane / T::TILE;
     const int bid0 = logical_block(p.xcd_map), split = bid0 % p.splits, bid = bid0 / p.splits;
@@ -25,32 +25,22 @@ __global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_fwd_kernel(Args p) {
     const Kept kept(p, z);
     const int b = kept.b;
     const int n = clamp_len(p.q_lens, b, p.Tq), m = clamp_len(p.kv_lens, b, p.Tk), off = m - n;
-    const int c0 = blk * COLS, wc0 = c0 + wave / RS * CW * T::TILE;       // first column of the workgroup / of this wave
+    const int c0 = blk * COLS, col = c0 + wave / RS * T::TILE + cl;       // first column of the workgroup, this lane's
     const int row_slots = p.D * T::ES / 16;
     const float c = fabsf(p.scale) * LOG2E;
 
-    typename T::Frag qf[CW][KS];
-    int head[CW], tok[CW];
+    typename T::Frag qf[KS];
+    int head, tok;
+    kept.col(p, col < kept.cols ? col : kept.cols - 1, head, tok);
+    ld_kept<DT, KS>(qf, p.q.p + b * p.q.b + head * p.q.h + (tok < n ? tok : (n > 0 ? n - 1 : 0)) * p.q.t, row_slots, g);
+    if (p.scale < 0.f) {
 #pragma unroll
-    for (int cw = 0; cw < CW; ++cw) {
-        const int col = wc0 + cw * T::TILE + cl;
-        kept.col(p, col < kept.cols ? col : kept.cols - 1, head[cw], tok[cw]);
-        const int row = tok[cw] < n ? tok[cw] : (n > 0 ? n - 1 : 0);
-        ld_kept<DT, KS>(qf[cw], p.q.p + b * p.q.b + head[cw] * p.q.h + row * p.q.t, row_slots, g);
-        if (p.scale < 0.f) {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) qf[cw][ks] = -qf[cw][ks];
-        }
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = -qf[ks];
     }
-    typename T::Acc o[CW][ND];
-    float mx[CW], l[CW];
+    typename T::Acc o[ND];
+    float mx = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int cw = 0; cw < CW; ++cw) {
-        mx[cw] = -INFINITY;
-        l[cw] = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) o[cw][dt] = typename T::Acc{};
-    }
+    for (int dt = 0; dt < ND; ++dt) o[dt] = typename T::Acc{};
 
     // streamed rows: [begin, open) are seen by every column, [open, end) through the mask
     const int t0 = p.packed ? 0 : c0, t1 = p.packed ? p.Tq : c0 + COLS;
@@ -67,67 +57,44 @@ __global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_fwd_kernel(Args p) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (r0 + BM < end) st.issue(smem + (cur ^ 1) * St::STAGE, r0 + BM, m, 0, 0);
-        const char* stage = smem + cur * St::STAGE;
+        const char *Ks = smem + cur * St::STAGE + rw * T::ROWS * RB, *Vs = Ks + St::TILE_BYTES;
         cur ^= 1;
+        Score<DT> s{};
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int rr = (rw * RT + rt) * T::TILE;
-            const char *Ks = stage + rr * RB, *Vs = Ks + St::TILE_BYTES;
-            typename T::Acc s[CW];
+        for (int ks = 0; ks < KS; ++ks) mma_rows<DT, RB>(Ks, lane, ks, qf[ks], s);
+        if constexpr (masked.value) {
+            const int seen = min(end, p.causal ? tok + off + 1 : end) - r0 - rw * T::ROWS - 4 * g;
 #pragma unroll
-            for (int cw = 0; cw < CW; ++cw) s[cw] = typename T::Acc{};
+            for (int r = 0; r < s.N; ++r) s.set(r, reg_row<DT>(r) < seen ? s.get(r) : -INFINITY);
+        }
+        float mb = s.get(0);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const typename T::Frag a = ld_row<DT, RB>(Ks, lane, ks);
+        for (int r = 1; r < s.N; ++r) mb = fmaxf(mb, s.get(r));
+        mb = col_max<T::TILE>(mb);
+        const bool grow = mb * c > mx * c + 8.f;
+        if (__any(grow)) {
+            const float nm = grow ? mb : mx;
+            const float alpha = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx - nm) * c);
+            mx = nm;
+            l *= alpha;
 #pragma unroll
-                for (int cw = 0; cw < CW; ++cw) s[cw] = T::mma(a, qf[cw][ks], s[cw]);
-            }
-            if constexpr (masked.value) {
+            for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-                for (int cw = 0; cw < CW; ++cw) {
-                    const int seen = min(end, p.causal ? tok[cw] + off + 1 : end) - r0 - rr - 4 * g;
+                for (int r = 0; r < T::NR; ++r) o[dt][r] *= alpha;
+        }
+        const float mc = mx == -INFINITY ? 0.f : mx * c;
+        float sum = 0.f;
 #pragma unroll
-                    for (int r = 0; r < T::NR; ++r) s[cw][r] = reg_row<DT>(r) < seen ? s[cw][r] : -INFINITY;
-                }
-            }
+        for (int r = 0; r < s.N; ++r) {
+            s.set(r, __builtin_amdgcn_exp2f(fmaf(s.get(r), c, -mc)));
+            sum += s.get(r);
+        }
+        l += sum;
 #pragma unroll
-            for (int cw = 0; cw < CW; ++cw) {
-                float mb = s[cw][0];
+        for (int kk = 0; kk < NKK; ++kk) {
+            const typename T::Frag pf = s.pack(kk);
 #pragma unroll
-                for (int r = 1; r < T::NR; ++r) mb = fmaxf(mb, s[cw][r]);
-                mb = col_max<T::TILE>(mb);
-                const bool grow = mb * c > mx[cw] * c + 8.f;
-                if (__any(grow)) {
-                    const float nm = grow ? mb : mx[cw];
-                    const float alpha = mx[cw] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx[cw] - nm) * c);
-                    mx[cw] = nm;
-                    l[cw] *= alpha;
-#pragma unroll
-                    for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-                        for (int r = 0; r < T::NR; ++r) o[cw][dt][r] *= alpha;
-                }
-                const float mc = mx[cw] == -INFINITY ? 0.f : mx[cw] * c;
-                float sum = 0.f;
-#pragma unroll
-                for (int r = 0; r < T::NR; ++r) {
-                    s[cw][r] = __builtin_amdgcn_exp2f(fmaf(s[cw][r], c, -mc));
-                    sum += s[cw][r];
-                }
-                l[cw] += sum;
-            }
-#pragma unroll
-            for (int kk = 0; kk < NKK; ++kk) {
-                typename T::Frag pf[CW];
-#pragma unroll
-                for (int cw = 0; cw < CW; ++cw) pf[cw] = pack<DT>(s[cw], kk);
-#pragma unroll
-                for (int dt = 0; dt < ND; ++dt) {
-                    const typename T::Frag a = ld_tr<DT, RB>(Vs, lane, kk, dt);
-#pragma unroll
-                    for (int cw = 0; cw < CW; ++cw) o[cw][dt] = T::mma(a, pf[cw], o[cw][dt]);
-                }
-            }
+            for (int dt = 0; dt < ND; ++dt) o[dt] = T::mma(ld_tr<DT, RB>(Vs, lane, kk, dt), pf, o[dt]);
         }
         settle();
     };
@@ -135,42 +102,35 @@ __global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_fwd_kernel(Args p) {
     for (; r0 < open; r0 += BM) body(r0, no{});
     for (; r0 < end; r0 += BM) body(r0, yes{});
 
-    if constexpr (RS > 1) __syncthreads();
-#pragma unroll
-    for (int cw = 0; cw < CW; ++cw) {
-        const int col = wc0 + cw * T::TILE + cl;
-        float sum = col_sum<T::TILE>(l[cw]), top = mx[cw], mine = 1.f;
-        if constexpr (RS > 1) {
-            if (g == 0) {
-                ml[0][wave][cw * T::TILE + cl] = top;
-                ml[1][wave][cw * T::TILE + cl] = sum;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < RS; ++w) top = fmaxf(top, ml[0][wave - rw + w][cw * T::TILE + cl]);
-            const float tc = top == -INFINITY ? 0.f : top * c;
-            mine = __builtin_amdgcn_exp2f(mx[cw] * c - tc);
-            sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < RS; ++w) sum += ml[1][wave - rw + w][cw * T::TILE + cl] * __builtin_amdgcn_exp2f(ml[0][wave - rw + w][cw * T::TILE + cl] * c - tc);
+    float sum = col_sum<T::TILE>(l), top = mx, mine = 1.f;
+    if constexpr (RS > 1) {
+        if (g == 0) {
+            ml[0][wave][cl] = top;
+            ml[1][wave][cl] = sum;
         }
-        const bool some = tok[cw] < n && sum > 0.f;
-        const float inv = some ? 1.f / sum : 0.f, lse = some ? top * fabsf(p.scale) + logf(sum) : -INFINITY;
-        const bool out = col < kept.cols;
-        const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
-        char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head[cw] * p.w0.h + tok[cw] * p.w0.t;
-        join_units<DT, ND, RS>(o[cw], mine, smem, wave, rw, lane, [&](int u, f32x4 v) {
-            const int d = Units<DT, ND>::d(u, g);
-            if (!out || d >= p.D) return;
-            v = some ? v * inv : f32x4{};
-            if (p.splits > 1) *reinterpret_cast<f32x4*>(p.part0 + kr * p.D + d) = v;
-            else st4<DT>(row, d, v);
-        });
-        if (out && g == 0 && rw == 0) {
-            if (p.splits > 1) p.part_lse[kr] = lse;
-            else p.lse[((long long)b * p.Hq + head[cw]) * p.Tq + tok[cw]] = lse;
-        }
-        if constexpr (RS > 1 && CW > 1) __syncthreads();
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < RS; ++w) top = fmaxf(top, ml[0][wave - rw + w][cl]);
+        const float tc = top == -INFINITY ? 0.f : top * c;
+        mine = __builtin_amdgcn_exp2f(mx * c - tc);
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < RS; ++w) sum += ml[1][wave - rw + w][cl] * __builtin_amdgcn_exp2f(ml[0][wave - rw + w][cl] * c - tc);
+    }
+    const bool some = tok < n && sum > 0.f, out = col < kept.cols;
+    const float inv = some ? 1.f / sum : 0.f, lse = some ? top * fabsf(p.scale) + logf(sum) : -INFINITY;
+    const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
+    char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head * p.w0.h + tok * p.w0.t;
+    join_units<DT, ND, RS>(o, mine, smem, wave, rw, lane, [&](int u, f32x4 v) {
+        const int d = Units<DT, ND>::d(u, g);
+        if (!out || d >= p.D) return;
+        v = some ? v * inv : f32x4{};
+        if (p.splits > 1) *reinterpret_cast<f32x4*>(p.part0 + kr * p.D + d) = v;
+        else st4<DT>(row, d, v);
+    });
+    if (out && g == 0 && rw == 0) {
+        if (p.splits > 1) p.part_lse[kr] = lse;
+        else p.lse[((long long)b * p.Hq + head) * p.Tq + tok] = lse;
     }
 }
 
@@ -218,28 +178,28 @@ __global__ __launch_bounds__(256) void attn_lse_join_kernel(Args p) {
     if (d == 0) p.lse[((long long)kept.b * p.Hq + h) * p.Tq + t] = top > -INFINITY ? top + logf(sum) : -INFINITY;
 }
 
-template <int DT, int DP>
+template <int DTYPE, int DP>
 void launch_fwd(Args a, hipStream_t s) {
-    constexpr int TILE = Tr<DT>::TILE, WIDE = DP > 128 ? 2 : 4;
-    const QPlan pl = q_plan(a.B, a.Tq, a.Tk, a.Hq, a.Hkv, DP, TILE);
+    constexpr int DT = shape_of(DTYPE, DP), FEW = DP > 128 ? 2 : 4;
+    const QPlan pl = q_plan(DTYPE, a.B, a.Tq, a.Tk, a.Hq, a.Hkv, DP);
     a.packed = pl.packed;
     a.splits = pl.splits;
     a.split_rows = pl.split_rows;
     a.stripes = stripes_of((long long)a.B * (pl.packed ? a.Hkv : a.Hq));
-    if (pl.rs == 1) hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, 1, 1, 1>), dim3((unsigned)(pl.blocks * pl.splits)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, 1, WIDE, 1>), dim3((unsigned)(pl.blocks * pl.splits)), dim3(256), 0, s, a);
+    if (pl.rs == 1) hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, 1>), dim3((unsigned)(pl.blocks * pl.splits)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_lse_fwd_kernel<DT, DP, FEW>), dim3((unsigned)(pl.blocks * pl.splits)), dim3(256), 0, s, a);
     if (pl.splits > 1) {
         const long long items = (long long)a.B * a.Hq * a.Tq * (a.D / 4);
-        hipLaunchKernelGGL(attn_lse_join_kernel<DT>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(attn_lse_join_kernel<DTYPE>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, a);
     }
 }
-template <int DT>
+template <int DTYPE>
 void launch_fwd(const Args& a, hipStream_t s) {
-    if (a.D <= 32) launch_fwd<DT, 32>(a, s);
-    else if (a.D <= 64) launch_fwd<DT, 64>(a, s);
-    else if (a.D <= 96) launch_fwd<DT, 96>(a, s);
-    else if (a.D <= 128) launch_fwd<DT, 128>(a, s);
-    else launch_fwd<DT, 256>(a, s);
+    if (a.D <= 32) launch_fwd<DTYPE, 32>(a, s);
+    else if (a.D <= 64) launch_fwd<DTYPE, 64>(a, s);
+    else if (a.D <= 96) launch_fwd<DTYPE, 96>(a, s);
+    else if (a.D <= 128) launch_fwd<DTYPE, 128>(a, s);
+    else launch_fwd<DTYPE, 256>(a, s);
 }
 
 }  // namespace
@@ -273,7 +233,7 @@ int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void*
     DP_REQUIRE(Hq % Hkv == 0, "%s: %d query heads are not a multiple of %d key heads", fn, Hq, Hkv);
     DP_REQUIRE(D > 0 && D % 8 == 0 && D <= 256, "%s: the head dimension must be a multiple of 8 up to 256 (got %d)", fn, D);
     DP_REQUIRE(Tq <= (1 << 30) && Tk <= (1 << 30), "%s: at most 2^30 tokens (got %d, %d)", fn, Tq, Tk);
-    const int cols = dtype == 0 ? 64 : 128;       // a grid has fewer than 2^32 threads; the launch that keeps keys has up to two workgroups of 256 per block
+    const int cols = 4 * al::tile_of(dtype, al::padded_dim(D));       // a grid has fewer than 2^32 threads; the launch that keeps keys has up to two workgroups of 256 per block
     DP_REQUIRE((long long)B * Hq * ((Tq + cols - 1) / cols) < (1LL << 23) && (long long)B * Hkv * ((Tk + cols - 1) / cols) < (1LL << 23), "%s: too many blocks", fn);
     DP_REQUIRE(scale != 0.f && scale - scale == 0.f, "%s: the scale must be finite and not zero", fn);
     const int es = dtype == 0 ? 4 : 2;
@@ -294,7 +254,7 @@ int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void*
 
 extern "C" long long dp_attention_lse_workspace(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D) {
     if (dtype < 0 || dtype > 2 || B <= 0 || Tq <= 0 || Tk <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return 0;
-    const al::QPlan pl = al::q_plan(B, Tq, Tk, Hq, Hkv, al::padded_dim(D), dtype == 0 ? 16 : 32);
+    const al::QPlan pl = al::q_plan(dtype, B, Tq, Tk, Hq, Hkv, al::padded_dim(D));
     return pl.splits > 1 ? (long long)pl.splits * B * Hq * Tq * (D + 1) * 4 : 0;
 }
 

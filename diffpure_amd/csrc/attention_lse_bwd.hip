@@ -13,10 +13,10 @@ namespace {
 using namespace al;
 
 // dQ.  Workgroups, stages and RS as in the forward kernel.
-template <int DT, int DP, int CW, int RS, int RT>
-__global__ __launch_bounds__(256) AL_WAVES(DT && DP == 64 && RS == 1 ? 3 : DP <= 128 ? 2 : 1) void attn_lse_dq_kernel(Args p) {
+template <int DT, int DP, int RS>
+__global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP == 64 && RS == 1 ? 3 : 2) void attn_lse_dq_kernel(Args p) {
     using T = Tr<DT>;
-    constexpr int NW = 4, BM = RS * RT * T::TILE, RB = DP * T::ES, KS = DP / 16, ND = DP / T::TILE, NKK = T::TILE / 16, COLS = NW / RS * CW * T::TILE;
+    constexpr int NW = 4, BM = RS * T::ROWS, RB = DP * T::ES, KS = DP / T::KSTEP, ND = DP / T::TILE, NKK = T::ROWS / T::KROWS, COLS = NW / RS * T::TILE;
     using St = Stream<RB, T::ES, BM, NW>;
     __shared__ __attribute__((aligned(1024))) char smem[2 * St::STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -28,45 +28,35 @@ __global__ __launch_bounds__(256) AL_WAVES(DT && DP == 64 && RS == 1 ? 3 : DP <=
     const Kept kept(p, z);
     const int b = kept.b;
     const int n = clamp_len(p.q_lens, b, p.Tq), m = clamp_len(p.kv_lens, b, p.Tk), off = m - n;
-    const int c0 = blk * COLS, wc0 = c0 + wave / RS * CW * T::TILE;
+    const int c0 = blk * COLS, col = c0 + wave / RS * T::TILE + cl;
     const int row_slots = p.D * T::ES / 16;
     const float c = p.scale * LOG2E;
     const long long half = (long long)p.B * p.Hq * p.Tqp;
 
-    typename T::Frag qf[CW][KS], df[CW][KS];
-    typename T::Acc dq[CW][ND], nd[CW];
-    float l2[CW];
-    int head[CW], tok[CW];
+    typename T::Frag qf[KS], df[KS];
+    int head, tok;
+    kept.col(p, col < kept.cols ? col : kept.cols - 1, head, tok);
+    const int krow = tok < n ? tok : (n > 0 ? n - 1 : 0);
+    ld_kept<DT, KS>(qf, p.q.p + b * p.q.b + head * p.q.h + krow * p.q.t, row_slots, g);
+    ld_kept<DT, KS>(df, p.dout.p + b * p.dout.b + head * p.dout.h + krow * p.dout.t, row_slots, g);
+    float delta = 0.f;
+    {
+        typename T::Frag of[KS];
+        ld_kept<DT, KS>(of, p.o.p + b * p.o.b + head * p.o.h + krow * p.o.t, row_slots, g);
 #pragma unroll
-    for (int cw = 0; cw < CW; ++cw) {
-        const int col = wc0 + cw * T::TILE + cl;
-        kept.col(p, col < kept.cols ? col : kept.cols - 1, head[cw], tok[cw]);
-        const int row = tok[cw] < n ? tok[cw] : (n > 0 ? n - 1 : 0);
-        ld_kept<DT, KS>(qf[cw], p.q.p + b * p.q.b + head[cw] * p.q.h + row * p.q.t, row_slots, g);
-        ld_kept<DT, KS>(df[cw], p.dout.p + b * p.dout.b + head[cw] * p.dout.h + row * p.dout.t, row_slots, g);
-        float delta = 0.f;
-        {
-            typename T::Frag of[KS];
-            ld_kept<DT, KS>(of, p.o.p + b * p.o.b + head[cw] * p.o.h + row * p.o.t, row_slots, g);
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int j = 0; j < 16 / T::ES; ++j) delta = fmaf((float)df[cw][ks][j], (float)of[ks][j], delta);
-        }
-        delta = col_sum<T::TILE>(delta);
-        const long long at = (long long)b * p.Hq + head[cw];
-        const float lse = p.lse[at * p.Tq + row];
-        const bool some = tok[cw] < n && lse > -INFINITY;
-        l2[cw] = some ? lse * LOG2E - (float)T::PSHIFT : INFINITY;
-        if (!some) delta = 0.f;
-        if (g == 0 && rw == 0 && split == 0 && col < kept.cols) {
-            p.rows[at * p.Tqp + tok[cw]] = l2[cw];
-            p.rows[half + at * p.Tqp + tok[cw]] = -delta;
-        }
-#pragma unroll
-        for (int r = 0; r < T::NR; ++r) nd[cw][r] = -delta;
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) dq[cw][dt] = typename T::Acc{};
+            for (int j = 0; j < 16 / T::ES; ++j) delta = fmaf((float)df[ks][j], (float)of[ks][j], delta);
+    }
+    delta = col_sum<T::TILE>(delta);
+    const long long zh = (long long)b * p.Hq + head;
+    const float lse = p.lse[zh * p.Tq + krow];
+    const bool some = tok < n && lse > -INFINITY;
+    const float l2 = some ? lse * LOG2E - (float)T::PSHIFT : INFINITY;
+    if (!some) delta = 0.f;
+    if (g == 0 && rw == 0 && split == 0 && col < kept.cols) {
+        p.rows[zh * p.Tqp + tok] = l2;
+        p.rows[half + zh * p.Tqp + tok] = -delta;
     }
     if (blk == nblk - 1 && split == 0) {          // the rows that round Tq up: no such query
         const int pad = p.Tqp - p.Tq, heads = p.packed ? p.Hq / p.Hkv : 1;
@@ -76,6 +66,11 @@ __global__ __launch_bounds__(256) AL_WAVES(DT && DP == 64 && RS == 1 ? 3 : DP <=
             p.rows[half + at] = 0.f;
         }
     }
+    Score<DT> nd;                                 // dP starts from -delta
+    nd.fill(-delta);
+    typename T::Acc dq[ND];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) dq[dt] = typename T::Acc{};
 
     const int t0 = p.packed ? 0 : c0, t1 = p.packed ? p.Tq : c0 + COLS;
     int begin = split * p.split_rows, end = t0 < n ? m : 0, open;
@@ -91,55 +86,28 @@ __global__ __launch_bounds__(256) AL_WAVES(DT && DP == 64 && RS == 1 ? 3 : DP <=
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (r0 + BM < end) st.issue(smem + (cur ^ 1) * St::STAGE, r0 + BM, m, 0, 0);
-        const char* stage = smem + cur * St::STAGE;
+        const char *Ks = smem + cur * St::STAGE + rw * T::ROWS * RB, *Vs = Ks + St::TILE_BYTES;
         cur ^= 1;
+        Score<DT> s{}, ds = nd;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int rr = (rw * RT + rt) * T::TILE;
-            const char *Ks = stage + rr * RB, *Vs = Ks + St::TILE_BYTES;
-            typename T::Acc s[CW], ds[CW];
+        for (int ks = 0; ks < KS; ++ks) {
+            mma_rows<DT, RB>(Ks, lane, ks, qf[ks], s);
+            mma_rows<DT, RB>(Vs, lane, ks, df[ks], ds);
+        }
 #pragma unroll
-            for (int cw = 0; cw < CW; ++cw) {
-                s[cw] = typename T::Acc{};
-                ds[cw] = nd[cw];
-            }
+        for (int r = 0; r < s.N; ++r) s.set(r, __builtin_amdgcn_exp2f(fmaf(s.get(r), c, -l2)));
+        if constexpr (masked.value) {
+            const int seen = min(end, p.causal ? tok + off + 1 : end) - r0 - rw * T::ROWS - 4 * g;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const typename T::Frag ak = ld_row<DT, RB>(Ks, lane, ks), av = ld_row<DT, RB>(Vs, lane, ks);
+            for (int r = 0; r < s.N; ++r) s.set(r, reg_row<DT>(r) < seen ? s.get(r) : 0.f);
+        }
 #pragma unroll
-                for (int cw = 0; cw < CW; ++cw) {
-                    s[cw] = T::mma(ak, qf[cw][ks], s[cw]);
-                    ds[cw] = T::mma(av, df[cw][ks], ds[cw]);
-                }
-            }
+        for (int r = 0; r < s.N; ++r) ds.set(r, ds.get(r) * s.get(r));
 #pragma unroll
-            for (int cw = 0; cw < CW; ++cw)
+        for (int kk = 0; kk < NKK; ++kk) {
+            const typename T::Frag f = ds.pack(kk);
 #pragma unroll
-                for (int r = 0; r < T::NR; ++r) s[cw][r] = __builtin_amdgcn_exp2f(fmaf(s[cw][r], c, -l2[cw]));
-            if constexpr (masked.value) {
-#pragma unroll
-                for (int cw = 0; cw < CW; ++cw) {
-                    const int seen = min(end, p.causal ? tok[cw] + off + 1 : end) - r0 - rr - 4 * g;
-#pragma unroll
-                    for (int r = 0; r < T::NR; ++r) s[cw][r] = reg_row<DT>(r) < seen ? s[cw][r] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int cw = 0; cw < CW; ++cw)
-#pragma unroll
-                for (int r = 0; r < T::NR; ++r) ds[cw][r] *= s[cw][r];
-#pragma unroll
-            for (int kk = 0; kk < NKK; ++kk) {
-                typename T::Frag f[CW];
-#pragma unroll
-                for (int cw = 0; cw < CW; ++cw) f[cw] = pack<DT>(ds[cw], kk);
-#pragma unroll
-                for (int dt = 0; dt < ND; ++dt) {
-                    const typename T::Frag a = ld_tr<DT, RB>(Ks, lane, kk, dt);
-#pragma unroll
-                    for (int cw = 0; cw < CW; ++cw) dq[cw][dt] = T::mma(a, f[cw], dq[cw][dt]);
-                }
-            }
+            for (int dt = 0; dt < ND; ++dt) dq[dt] = T::mma(ld_tr<DT, RB>(Ks, lane, kk, dt), f, dq[dt]);
         }
         settle();
     };
@@ -147,41 +115,36 @@ __global__ __launch_bounds__(256) AL_WAVES(DT && DP == 64 && RS == 1 ? 3 : DP <=
     for (; r0 < open; r0 += BM) body(r0, no{});
     for (; r0 < end; r0 += BM) body(r0, yes{});
 
-    const float mul = p.scale / (float)(1 << T::PSHIFT);
-#pragma unroll
-    for (int cw = 0; cw < CW; ++cw) {
-        if constexpr (RS > 1) __syncthreads();
-        const int col = wc0 + cw * T::TILE + cl;
-        const bool out = col < kept.cols, some = tok[cw] < n;
-        const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
-        char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head[cw] * p.w0.h + tok[cw] * p.w0.t;
-        join_units<DT, ND, RS>(dq[cw], mul, smem, wave, rw, lane, [&](int u, f32x4 v) {
-            const int d = Units<DT, ND>::d(u, g);
-            if (!out || d >= p.D) return;
-            if (!some) v = f32x4{};
-            if (p.splits > 1) *reinterpret_cast<f32x4*>(p.part0 + kr * p.D + d) = v;
-            else st4<DT>(row, d, v);
-        });
-    }
+    if constexpr (RS > 1) __syncthreads();
+    const bool out = col < kept.cols;
+    const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
+    char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head * p.w0.h + tok * p.w0.t;
+    join_units<DT, ND, RS>(dq, p.scale / (float)(1 << T::PSHIFT), smem, wave, rw, lane, [&](int u, f32x4 v) {
+        const int d = Units<DT, ND>::d(u, g);
+        if (!out || d >= p.D) return;
+        if (tok >= n) v = f32x4{};
+        if (p.splits > 1) *reinterpret_cast<f32x4*>(p.part0 + kr * p.D + d) = v;
+        else st4<DT>(row, d, v);
+    });
 }
 
 // dK and dV: keys are kept, the queries of every head of the group stream by, one head after the other.  WHAT: 1 dK, 2 dV, 3 both.
-template <int DT, int DP, int CW, int RS, int RT> struct Dkv {
-    static constexpr int NW = 4, BM = RS * RT * Tr<DT>::TILE, RB = DP * Tr<DT>::ES;
+template <int DT, int DP, int RS> struct Dkv {
+    static constexpr int NW = 4, BM = RS * Tr<DT>::ROWS, RB = DP * Tr<DT>::ES, STATS = 2 * BM < 64 ? 64 : 2 * BM;
     using St = Stream<RB, Tr<DT>::ES, BM, NW>;
     struct Shared {
         char stage[2 * St::STAGE];
-        float rows[2][2][BM];             // stage: log-sum-exp, -delta of the streamed queries
+        float rows[2][STATS];             // stage: BM log-sum-exps, then BM -delta of the streamed queries (copied by whole waves)
     };
 };
-template <int DT, int DP, int CW, int RS, int RT, int WHAT>
-__device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<DT, DP, CW, RS, RT>::Shared& sh) {
+template <int DT, int DP, int RS, int WHAT>
+__device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<DT, DP, RS>::Shared& sh) {
     using T = Tr<DT>;
-    using K = Dkv<DT, DP, CW, RS, RT>;
+    using K = Dkv<DT, DP, RS>;
     using St = typename K::St;
-    constexpr int NW = K::NW, BM = K::BM, RB = K::RB, KS = DP / 16, ND = DP / T::TILE, NKK = T::TILE / 16, COLS = NW / RS * CW * T::TILE;
+    constexpr int NW = K::NW, BM = K::BM, RB = K::RB, KS = DP / T::KSTEP, ND = DP / T::TILE, NKK = T::ROWS / T::KROWS, COLS = NW / RS * T::TILE;
     constexpr bool DK = WHAT & 1, DV = WHAT & 2;
-    static_assert(BM % 32 == 0 && BM <= 128, "whole waves copy the rows' statistics, of which a multiple of 128 exist");
+    static_assert(128 % BM == 0 && K::STATS <= 256, "the statistics exist for a multiple of 128 rows");
     char* smem = sh.stage;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = wave % RS, cl = lane & (T::TILE - 1), g = lane / T::TILE;
@@ -191,22 +154,19 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
     if (z >= p.B * p.Hkv) return;
     const int b = z / p.Hkv, hk = z - b * p.Hkv;
     const int n = clamp_len(p.q_lens, b, p.Tq), m = clamp_len(p.kv_lens, b, p.Tk), off = m - n;
-    const int c0 = blk * COLS, wc0 = c0 + wave / RS * CW * T::TILE;
+    const int c0 = blk * COLS, col = c0 + wave / RS * T::TILE + cl;
     const int row_slots = p.D * T::ES / 16;
     const float c = p.scale * LOG2E;
 
-    typename T::Frag kf[CW][KS], vf[CW][DK ? KS : 1];
-    typename T::Acc dk[CW][DK ? ND : 1], dv[CW][DV ? ND : 1];
+    typename T::Frag kf[KS], vf[DK ? KS : 1];
+    typename T::Acc dk[DK ? ND : 1], dv[DV ? ND : 1];
+    const int krow = col < m ? col : (m > 0 ? m - 1 : 0);
+    ld_kept<DT, KS>(kf, p.k.p + b * p.k.b + hk * p.k.h + krow * p.k.t, row_slots, g);
+    if constexpr (DK) ld_kept<DT, KS>(vf, p.v.p + b * p.v.b + hk * p.v.h + krow * p.v.t, row_slots, g);
 #pragma unroll
-    for (int cw = 0; cw < CW; ++cw) {
-        const int col = wc0 + cw * T::TILE + cl, row = col < m ? col : (m > 0 ? m - 1 : 0);
-        ld_kept<DT, KS>(kf[cw], p.k.p + b * p.k.b + hk * p.k.h + row * p.k.t, row_slots, g);
-        if constexpr (DK) ld_kept<DT, KS>(vf[cw], p.v.p + b * p.v.b + hk * p.v.h + row * p.v.t, row_slots, g);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) {
-            if constexpr (DK) dk[cw][dt] = typename T::Acc{};
-            if constexpr (DV) dv[cw][dt] = typename T::Acc{};
-        }
+    for (int dt = 0; dt < ND; ++dt) {
+        if constexpr (DK) dk[dt] = typename T::Acc{};
+        if constexpr (DV) dv[dt] = typename T::Acc{};
     }
 
     // Streamed rows of each head: [begin, open) through the causal mask, [open, end) see every column.  A split launch cuts a block's own rows into equal
@@ -222,11 +182,11 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
     else open = begin;
     St st;
     st.init(p.q.p + b * p.q.b + hk * group * p.q.h, p.q.t, p.dout.p + b * p.dout.b + hk * group * p.dout.h, p.dout.t, row_slots, wave, lane);
-    // lane t < 2 BM of the workgroup copies one value of a tile: log-sum-exp (t < BM) or -delta of query t % BM
-    const float* mine = p.rows + ((long long)b * p.Hq + hk * group) * p.Tqp + (tid < BM ? tid : (long long)p.B * p.Hq * p.Tqp + tid - BM);
+    const int stat = tid & (2 * BM - 1);
+    const float* mine = p.rows + ((long long)b * p.Hq + hk * group) * p.Tqp + (stat < BM ? stat : (long long)p.B * p.Hq * p.Tqp + stat - BM);
     auto issue = [&](int stage, int head, int r0) {
         st.issue(smem + stage * St::STAGE, r0, n, head * p.q.h, head * p.dout.h);
-        if (wave * 64 < 2 * BM) AL_GLDS(mine + (long long)head * p.Tqp + r0, reinterpret_cast<char*>(&sh.rows[stage][0][0]) + wave * 256, 4);
+        if (wave * 64 < K::STATS) AL_GLDS(mine + (long long)head * p.Tqp + r0, reinterpret_cast<char*>(sh.rows[stage]) + wave * 256, 4);
     };
     // Rows are taken from the last one down: a causal mask lets the blocks of a head begin at different rows but end at the same one, and the blocks that run
     // at a time share what they stream (in L2) only while they stand at the same row.
@@ -237,79 +197,46 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
         __syncthreads();
         const bool wrap = r0 == begin;
         if (!wrap || head + 1 < group) issue(cur ^ 1, wrap ? head + 1 : head, wrap ? last : r0 - BM);
-        const char* stage = smem + cur * St::STAGE;
-        const float(*rs)[BM] = sh.rows[cur];
+        const char *Qs = smem + cur * St::STAGE + rw * T::ROWS * RB, *Ds = Qs + St::TILE_BYTES;
+        const float* rs = sh.rows[cur] + rw * T::ROWS + 4 * g;
         cur ^= 1;
+        Score<DT> l2, s{}, ds{};
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int rr = (rw * RT + rt) * T::TILE;
-            const char *Qs = stage + rr * RB, *Ds = Qs + St::TILE_BYTES;
-            typename T::Acc l2, nd;
+        for (int r = 0; r < s.N; r += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(rs + reg_row<DT>(r));
+            f32x4 y = {};
+            if constexpr (DK) y = *reinterpret_cast<const f32x4*>(rs + BM + reg_row<DT>(r));
 #pragma unroll
-            for (int r = 0; r < T::NR; r += 4) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(&rs[0][rr + r * T::G + 4 * g]);
-                f32x4 y = {};
-                if constexpr (DK) y = *reinterpret_cast<const f32x4*>(&rs[1][rr + r * T::G + 4 * g]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    l2[r + j] = x[j];
-                    nd[r + j] = y[j];
-                }
+            for (int j = 0; j < 4; ++j) {
+                l2.set(r + j, x[j]);
+                ds.set(r + j, y[j]);
             }
-            typename T::Acc s[CW], ds[CW];
+        }
 #pragma unroll
-            for (int cw = 0; cw < CW; ++cw) {
-                s[cw] = typename T::Acc{};
-                ds[cw] = nd;
-            }
+        for (int ks = 0; ks < KS; ++ks) {
+            mma_rows<DT, RB>(Qs, lane, ks, kf[ks], s);
+            if constexpr (DK) mma_rows<DT, RB>(Ds, lane, ks, vf[ks], ds);
+        }
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const typename T::Frag aq = ld_row<DT, RB>(Qs, lane, ks);
+        for (int r = 0; r < s.N; ++r) s.set(r, __builtin_amdgcn_exp2f(fmaf(s.get(r), c, -l2.get(r))));
+        if constexpr (masked.value) {
+            const int first = col - off - r0 - rw * T::ROWS - 4 * g;       // first row of the tile that sees this key
 #pragma unroll
-                for (int cw = 0; cw < CW; ++cw) s[cw] = T::mma(aq, kf[cw][ks], s[cw]);
-                if constexpr (DK) {
-                    const typename T::Frag ad = ld_row<DT, RB>(Ds, lane, ks);
+            for (int r = 0; r < s.N; ++r) s.set(r, reg_row<DT>(r) >= first ? s.get(r) : 0.f);
+        }
+        if constexpr (DK) {
 #pragma unroll
-                    for (int cw = 0; cw < CW; ++cw) ds[cw] = T::mma(ad, vf[cw][ks], ds[cw]);
-                }
-            }
+            for (int r = 0; r < s.N; ++r) ds.set(r, ds.get(r) * s.get(r));
+        }
 #pragma unroll
-            for (int cw = 0; cw < CW; ++cw)
+        for (int kk = 0; kk < NKK; ++kk) {
+            typename T::Frag pf, sf;
+            if constexpr (DV) pf = s.pack(kk);
+            if constexpr (DK) sf = ds.pack(kk);
 #pragma unroll
-                for (int r = 0; r < T::NR; ++r) s[cw][r] = __builtin_amdgcn_exp2f(fmaf(s[cw][r], c, -l2[r]));
-            if constexpr (masked.value) {
-#pragma unroll
-                for (int cw = 0; cw < CW; ++cw) {
-                    const int first = wc0 + cw * T::TILE + cl - off - r0 - rr - 4 * g;       // first row of the tile that sees this key
-#pragma unroll
-                    for (int r = 0; r < T::NR; ++r) s[cw][r] = reg_row<DT>(r) >= first ? s[cw][r] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int cw = 0; cw < CW; ++cw)
-#pragma unroll
-                for (int r = 0; r < T::NR; ++r) ds[cw][r] *= s[cw][r];
-#pragma unroll
-            for (int kk = 0; kk < NKK; ++kk) {
-                typename T::Frag pf[CW], sf[CW];
-#pragma unroll
-                for (int cw = 0; cw < CW; ++cw) {
-                    if constexpr (DV) pf[cw] = pack<DT>(s[cw], kk);
-                    if constexpr (DK) sf[cw] = pack<DT>(ds[cw], kk);
-                }
-#pragma unroll
-                for (int dt = 0; dt < ND; ++dt) {
-                    if constexpr (DV) {
-                        const typename T::Frag ad = ld_tr<DT, RB>(Ds, lane, kk, dt);
-#pragma unroll
-                        for (int cw = 0; cw < CW; ++cw) dv[cw][dt] = T::mma(ad, pf[cw], dv[cw][dt]);
-                    }
-                    if constexpr (DK) {
-                        const typename T::Frag aq = ld_tr<DT, RB>(Qs, lane, kk, dt);
-#pragma unroll
-                        for (int cw = 0; cw < CW; ++cw) dk[cw][dt] = T::mma(aq, sf[cw], dk[cw][dt]);
-                    }
-                }
+            for (int dt = 0; dt < ND; ++dt) {
+                if constexpr (DV) dv[dt] = T::mma(ld_tr<DT, RB>(Ds, lane, kk, dt), pf, dv[dt]);
+                if constexpr (DK) dk[dt] = T::mma(ld_tr<DT, RB>(Qs, lane, kk, dt), sf, dk[dt]);
             }
         }
         settle();
@@ -324,37 +251,33 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
     }
 
     const float pm = 1.f / (float)(1 << T::PSHIFT);
-#pragma unroll
-    for (int cw = 0; cw < CW; ++cw) {
-        const int col = wc0 + cw * T::TILE + cl;
-        const bool out = col < p.Tk, some = col < m;
-        const long long kr = ((long long)split * p.B * p.Hkv + z) * p.Tk + col;
-        auto put = [&](const Ten& w, float* part, int u, f32x4 v) {
-            const int d = Units<DT, ND>::d(u, g);
-            if (!out || d >= p.D) return;
-            if (!some) v = f32x4{};
-            if (p.splits > 1) *reinterpret_cast<f32x4*>(part + kr * p.D + d) = v;
-            else st4<DT>(const_cast<char*>(w.p) + b * w.b + hk * w.h + col * w.t, d, v);
-        };
-        if constexpr (DK) {
-            if constexpr (RS > 1) __syncthreads();
-            join_units<DT, ND, RS>(dk[cw], p.scale * pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w0, p.part0, u, v); });
-        }
-        if constexpr (DV) {
-            if constexpr (RS > 1) __syncthreads();
-            join_units<DT, ND, RS>(dv[cw], pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w1, p.part1, u, v); });
-        }
+    const bool out = col < p.Tk, some = col < m;
+    const long long kr = ((long long)split * p.B * p.Hkv + z) * p.Tk + col;
+    auto put = [&](const Ten& w, float* part, int u, f32x4 v) {
+        const int d = Units<DT, ND>::d(u, g);
+        if (!out || d >= p.D) return;
+        if (!some) v = f32x4{};
+        if (p.splits > 1) *reinterpret_cast<f32x4*>(part + kr * p.D + d) = v;
+        else st4<DT>(const_cast<char*>(w.p) + b * w.b + hk * w.h + col * w.t, d, v);
+    };
+    if constexpr (DK) {
+        if constexpr (RS > 1) __syncthreads();
+        join_units<DT, ND, RS>(dk, p.scale * pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w0, p.part0, u, v); });
+    }
+    if constexpr (DV) {
+        if constexpr (RS > 1) __syncthreads();
+        join_units<DT, ND, RS>(dv, pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w1, p.part1, u, v); });
     }
 }
 
-template <int DT, int DP, int CW, int RS, int RT>
-__global__ __launch_bounds__(256) AL_WAVES(DP > 128 ? 1 : DT && DP == 64 && RS == 1 ? 3 : 2) void attn_lse_dkv_kernel(Args p) {
-    __shared__ __attribute__((aligned(1024))) typename Dkv<DT, DP, CW, RS, RT>::Shared sh;
+template <int DT, int DP, int RS>
+__global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP == 64 && RS == 1 ? 3 : 2) void attn_lse_dkv_kernel(Args p) {
+    __shared__ __attribute__((aligned(1024))) typename Dkv<DT, DP, RS>::Shared sh;
     const int bid = logical_block(p.xcd_map);
-    if constexpr (two_roles(DP)) {
-        if (bid & 1) dkv_block<DT, DP, CW, RS, RT, 2>(p, bid >> 1, sh);
-        else dkv_block<DT, DP, CW, RS, RT, 1>(p, bid >> 1, sh);
-    } else dkv_block<DT, DP, CW, RS, RT, 3>(p, bid, sh);
+    if constexpr (two_roles(DT, DP)) {
+        if (bid & 1) dkv_block<DT, DP, RS, 2>(p, bid >> 1, sh);
+        else dkv_block<DT, DP, RS, 1>(p, bid >> 1, sh);
+    } else dkv_block<DT, DP, RS, 3>(p, bid, sh);
 }
 
 // sums of the ranges of a split launch, in their order: part [split][rows][D] -> rows of a [B, T, H, D] tensor.  Packed as the kept queries are, or plain
@@ -382,55 +305,55 @@ __global__ __launch_bounds__(256) void attn_lse_sum_kernel(Args p, int keys) {
     }
 }
 
-template <int DT, int DP>
+template <int DTYPE, int DP>
 void launch_bwd(const Args& a, const Ten& dq, const Ten& dk, const Ten& dv, hipStream_t s) {
-    constexpr int TILE = Tr<DT>::TILE, WIDE = DP > 128 ? 2 : 4, RT = DT == 0 ? 2 : 1;
+    constexpr int DT = shape_of(DTYPE, DP), FEW = DP > 128 ? 2 : 4;
     const dim3 wg(256);
     Args x = a;
     x.w0 = dq;
-    const QPlan pq = q_plan(a.B, a.Tq, a.Tk, a.Hq, a.Hkv, DP, TILE);
+    const QPlan pq = q_plan(DTYPE, a.B, a.Tq, a.Tk, a.Hq, a.Hkv, DP);
     x.packed = pq.packed;
     x.splits = pq.splits;
     x.split_rows = pq.split_rows;
     x.stripes = stripes_of((long long)a.B * (pq.packed ? a.Hkv : a.Hq));
     const dim3 gq((unsigned)(pq.blocks * pq.splits));
-    if (pq.rs == 1) hipLaunchKernelGGL((attn_lse_dq_kernel<DT, DP, 1, 1, 1>), gq, wg, 0, s, x);
-    else hipLaunchKernelGGL((attn_lse_dq_kernel<DT, DP, 1, WIDE, 1>), gq, wg, 0, s, x);
+    if (pq.rs == 1) hipLaunchKernelGGL((attn_lse_dq_kernel<DT, DP, 1>), gq, wg, 0, s, x);
+    else hipLaunchKernelGGL((attn_lse_dq_kernel<DT, DP, FEW>), gq, wg, 0, s, x);
     if (pq.splits > 1) {
         const long long items = (long long)a.B * a.Hq * a.Tq * (a.D / 4);
-        hipLaunchKernelGGL(attn_lse_sum_kernel<DT>, dim3((unsigned)((items + 255) / 256)), wg, 0, s, x, 0);
+        hipLaunchKernelGGL(attn_lse_sum_kernel<DTYPE>, dim3((unsigned)((items + 255) / 256)), wg, 0, s, x, 0);
     }
     x.w0 = dk;
     x.w1 = dv;
     x.packed = 0;
-    const KPlan pk = k_plan(a.B, a.Tq, a.Tk, a.Hkv, DP, TILE, DT == 0, a.causal);
+    const KPlan pk = k_plan(DTYPE, a.B, a.Tq, a.Tk, a.Hkv, DP, a.causal);
     x.stripes = stripes_of((long long)a.B * a.Hkv);
     x.splits = pk.splits;
     x.part1 = x.part0 + (long long)pk.splits * a.B * a.Hkv * a.Tk * a.D;
-    const dim3 gk((unsigned)(pk.blocks * pk.splits * (two_roles(DP) ? 2 : 1)));
-    if (pk.rs == 1) hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, 1, 1, RT>), gk, wg, 0, s, x);
-    else hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, 1, WIDE, 1>), gk, wg, 0, s, x);
+    const dim3 gk((unsigned)(pk.blocks * pk.splits * (two_roles(DTYPE, DP) ? 2 : 1)));
+    if (pk.rs == 1) hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, 1>), gk, wg, 0, s, x);
+    else hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, FEW>), gk, wg, 0, s, x);
     if (pk.splits > 1) {
         const long long items = (long long)a.B * a.Hkv * a.Tk * (a.D / 4);
-        hipLaunchKernelGGL(attn_lse_sum_kernel<DT>, dim3((unsigned)((items + 255) / 256)), wg, 0, s, x, 1);
+        hipLaunchKernelGGL(attn_lse_sum_kernel<DTYPE>, dim3((unsigned)((items + 255) / 256)), wg, 0, s, x, 1);
     }
 }
-template <int DT>
+template <int DTYPE>
 void launch_bwd(const Args& a, const Ten& dq, const Ten& dk, const Ten& dv, hipStream_t s) {
-    if (a.D <= 32) launch_bwd<DT, 32>(a, dq, dk, dv, s);
-    else if (a.D <= 64) launch_bwd<DT, 64>(a, dq, dk, dv, s);
-    else if (a.D <= 96) launch_bwd<DT, 96>(a, dq, dk, dv, s);
-    else if (a.D <= 128) launch_bwd<DT, 128>(a, dq, dk, dv, s);
-    else launch_bwd<DT, 256>(a, dq, dk, dv, s);
+    if (a.D <= 32) launch_bwd<DTYPE, 32>(a, dq, dk, dv, s);
+    else if (a.D <= 64) launch_bwd<DTYPE, 64>(a, dq, dk, dv, s);
+    else if (a.D <= 96) launch_bwd<DTYPE, 96>(a, dq, dk, dv, s);
+    else if (a.D <= 128) launch_bwd<DTYPE, 128>(a, dq, dk, dv, s);
+    else launch_bwd<DTYPE, 256>(a, dq, dk, dv, s);
 }
 
 }  // namespace
 
 extern "C" long long dp_attention_lse_bwd_workspace(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D) {
     if (dtype < 0 || dtype > 2 || B <= 0 || Tq <= 0 || Tk <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return 0;
-    const int tile = dtype == 0 ? 16 : 32, DP = al::padded_dim(D);
-    const al::QPlan pq = al::q_plan(B, Tq, Tk, Hq, Hkv, DP, tile);
-    const al::KPlan pk = al::k_plan(B, Tq, Tk, Hkv, DP, tile, dtype == 0, 1), pk0 = al::k_plan(B, Tq, Tk, Hkv, DP, tile, dtype == 0, 0);
+    const int DP = al::padded_dim(D);
+    const al::QPlan pq = al::q_plan(dtype, B, Tq, Tk, Hq, Hkv, DP);
+    const al::KPlan pk = al::k_plan(dtype, B, Tq, Tk, Hkv, DP, 1), pk0 = al::k_plan(dtype, B, Tq, Tk, Hkv, DP, 0);
     const long long rows = 2LL * B * Hq * ((Tq + 127LL) / 128 * 128);
     const long long q = pq.splits > 1 ? (long long)pq.splits * B * Hq * Tq * D : 0;
     const int ks = pk.splits > pk0.splits ? pk.splits : pk0.splits;
