@@ -287,11 +287,11 @@ __device__ __forceinline__ void join_units(const typename Tr<DT>::Acc (&acc)[ND]
     using U = Units<DT, ND>;
     if constexpr (RS == 1) {
 #pragma unroll
-        for (int u = 0; u < U::N; ++u) sink(u, U::get(acc, u) * mul);
+        for (int u = 0; u < U::N; ++u) sink(u, mul != 0.f ? U::get(acc, u) * mul : f32x4{});
     } else {
         f32x4* mine = reinterpret_cast<f32x4*>(smem) + (long long)wave * U::N * 64 + lane;
 #pragma unroll
-        for (int u = 0; u < U::N; ++u) mine[u * 64] = U::get(acc, u) * mul;
+        for (int u = 0; u < U::N; ++u) mine[u * 64] = mul != 0.f ? U::get(acc, u) * mul : f32x4{};
         __syncthreads();
         const f32x4* first = reinterpret_cast<const f32x4*>(smem) + (long long)(wave - rw) * U::N * 64 + lane;
         for (int u = rw; u < U::N; u += RS) {
@@ -300,6 +300,35 @@ __device__ __forceinline__ void join_units(const typename Tr<DT>::Acc (&acc)[ND]
             for (int w = 1; w < RS; ++w) s += first[(w * U::N + u) * 64];
             sink(u, s);
         }
+    }
+}
+
+// The kept columns of a wave, [d][column] in its accumulators, to rows of global memory: through LDS (smem: TILE rows of RB bytes of this wave's own), so that
+// a row leaves in whole 16-byte pieces of consecutive lanes.  Straight from the accumulators a store instruction writes 8 bytes here and there of 32 rows.
+// row_of(i) -> address of column i's row, or null.  A barrier must lie before the call (the region held streamed rows).
+template <int DT, int ND, int RB, typename Row>
+__device__ __forceinline__ void store_cols(const typename Tr<DT>::Acc (&acc)[ND], float mul, char* smem, int lane, int row_slots, Row row_of) {
+    using T = Tr<DT>;
+    using U = Units<DT, ND>;
+    using L = Lds<RB, T::ES>;
+    const int cl = lane & (T::TILE - 1), g = lane / T::TILE;
+#pragma unroll
+    for (int u = 0; u < U::N; ++u) {
+        const f32x4 v = mul != 0.f ? U::get(acc, u) * mul : f32x4{};        // (0: a row that is to be zero whatever its accumulator holds)
+        const int byte = U::d(u, g) * T::ES;
+        typename T::E4 e;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = (typename T::E)v[j];
+        *reinterpret_cast<typename T::E4*>(smem + L::at(cl, byte >> 4) + (byte & 8)) = e;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    constexpr int ITEMS = T::TILE * L::SLOTS;
+#pragma unroll
+    for (int i = 0; i < ITEMS / 64; ++i) {
+        const int id = i * 64 + lane, row = id / L::SLOTS, slot = id % L::SLOTS;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(smem + L::at(row, slot));
+        char* to = row_of(row);
+        if (to && slot < row_slots) *reinterpret_cast<f32x4*>(to + slot * 16) = v;
     }
 }
 

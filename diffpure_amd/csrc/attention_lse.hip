@@ -121,7 +121,15 @@ __global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_fwd_kernel(Args p) {
     const float inv = some ? 1.f / sum : 0.f, lse = some ? top * fabsf(p.scale) + logf(sum) : -INFINITY;
     const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
     char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head * p.w0.h + tok * p.w0.t;
-    join_units<DT, ND, RS>(o, mine, smem, wave, rw, lane, [&](int u, f32x4 v) {
+    if (RS == 1 && p.splits == 1) {
+        __syncthreads();
+        const int first = c0 + wave * T::TILE;
+        store_cols<DT, ND, RB>(o, inv, smem + wave * T::TILE * RB, lane, row_slots, [&](int i) -> char* {
+            int h, t;
+            kept.col(p, min(first + i, kept.cols - 1), h, t);
+            return first + i < kept.cols ? const_cast<char*>(p.w0.p) + b * p.w0.b + h * p.w0.h + t * p.w0.t : nullptr;
+        });
+    } else join_units<DT, ND, RS>(o, mine, smem, wave, rw, lane, [&](int u, f32x4 v) {
         const int d = Units<DT, ND>::d(u, g);
         if (!out || d >= p.D) return;
         v = some ? v * inv : f32x4{};

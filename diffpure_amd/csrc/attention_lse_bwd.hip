@@ -119,10 +119,18 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     const bool out = col < kept.cols;
     const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
     char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head * p.w0.h + tok * p.w0.t;
-    join_units<DT, ND, RS>(dq, p.scale / (float)(1 << T::PSHIFT), smem, wave, rw, lane, [&](int u, f32x4 v) {
+    const float mul = tok < n ? p.scale / (float)(1 << T::PSHIFT) : 0.f;
+    if (RS == 1 && p.splits == 1) {
+        __syncthreads();
+        const int first = c0 + wave * T::TILE;
+        store_cols<DT, ND, RB>(dq, mul, smem + wave * T::TILE * RB, lane, row_slots, [&](int i) -> char* {
+            int h, t;
+            kept.col(p, min(first + i, kept.cols - 1), h, t);
+            return first + i < kept.cols ? const_cast<char*>(p.w0.p) + b * p.w0.b + h * p.w0.h + t * p.w0.t : nullptr;
+        });
+    } else join_units<DT, ND, RS>(dq, mul, smem, wave, rw, lane, [&](int u, f32x4 v) {
         const int d = Units<DT, ND>::d(u, g);
         if (!out || d >= p.D) return;
-        if (tok >= n) v = f32x4{};
         if (p.splits > 1) *reinterpret_cast<f32x4*>(p.part0 + kr * p.D + d) = v;
         else st4<DT>(row, d, v);
     });
@@ -250,24 +258,25 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
         }
     }
 
-    const float pm = 1.f / (float)(1 << T::PSHIFT);
-    const bool out = col < p.Tk, some = col < m;
+    const bool out = col < p.Tk;
+    const float pm = col < m ? 1.f / (float)(1 << T::PSHIFT) : 0.f;
     const long long kr = ((long long)split * p.B * p.Hkv + z) * p.Tk + col;
-    auto put = [&](const Ten& w, float* part, int u, f32x4 v) {
-        const int d = Units<DT, ND>::d(u, g);
-        if (!out || d >= p.D) return;
-        if (!some) v = f32x4{};
-        if (p.splits > 1) *reinterpret_cast<f32x4*>(part + kr * p.D + d) = v;
-        else st4<DT>(const_cast<char*>(w.p) + b * w.b + hk * w.h + col * w.t, d, v);
+    auto put = [&](const typename T::Acc(&acc)[ND], float mul, const Ten& w, float* part) {
+        __syncthreads();
+        if (RS == 1 && p.splits == 1) {
+            const int first = c0 + wave * T::TILE;
+            store_cols<DT, ND, RB>(acc, mul, smem + wave * T::TILE * RB, lane, row_slots, [&](int i) -> char* {
+                return first + i < p.Tk ? const_cast<char*>(w.p) + b * w.b + hk * w.h + (first + i) * w.t : nullptr;
+            });
+        } else join_units<DT, ND, RS>(acc, mul, smem, wave, rw, lane, [&](int u, f32x4 v) {
+            const int d = Units<DT, ND>::d(u, g);
+            if (!out || d >= p.D) return;
+            if (p.splits > 1) *reinterpret_cast<f32x4*>(part + kr * p.D + d) = v;
+            else st4<DT>(const_cast<char*>(w.p) + b * w.b + hk * w.h + col * w.t, d, v);
+        });
     };
-    if constexpr (DK) {
-        if constexpr (RS > 1) __syncthreads();
-        join_units<DT, ND, RS>(dk, p.scale * pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w0, p.part0, u, v); });
-    }
-    if constexpr (DV) {
-        if constexpr (RS > 1) __syncthreads();
-        join_units<DT, ND, RS>(dv, pm, smem, wave, rw, lane, [&](int u, f32x4 v) { put(p.w1, p.part1, u, v); });
-    }
+    if constexpr (DK) put(dk, p.scale * pm, p.w0, p.part0);
+    if constexpr (DV) put(dv, pm, p.w1, p.part1);
 }
 
 template <int DT, int DP, int RS>
