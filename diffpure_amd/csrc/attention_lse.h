@@ -438,9 +438,10 @@ inline QPlan q_plan(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int DP) {
 
 // The same for the launch that keeps keys (dK, dV).  Its partial sums are as large as 2 * splits results, so it is split for causal launches (whose
 // blocks differ in length) and for those that would leave CUs without a workgroup.
-// Above 64 channels (tiles of 32 columns, fp32) the two gradients are formed by different workgroups, each of which recomputes the scores: a wave that
-// holds both has 64 accumulators more and leaves no room for a second wave on its SIMD (8191 causal, heads of 128: 1434 us together, 1160 us apart).
-constexpr bool two_roles(int dtype, int DP) { return DP > 64 && shape_of(dtype, DP) < 3; }
+// Above 64 channels the two gradients are formed by different workgroups, each of which recomputes the scores: a wave that holds both has 64 accumulators
+// more and leaves no room for a second wave on its SIMD (8191 causal, heads of 128: 1434 us together, 1160 us apart; 128 heads of 256 channels x 256: 78.6 and
+// 76.4 us; heads of 64, where both fit: 182 us together for 32 x 1024 x 8 heads, and 5 products instead of 4 apart).
+constexpr bool two_roles(int DP) { return DP > 64; }
 
 struct KPlan {
     int rs, splits;
@@ -449,7 +450,7 @@ struct KPlan {
 inline KPlan k_plan(int dtype, int B, int Tq, int Tk, int Hkv, int DP, int causal) {
     KPlan pl;
     const long long heads = (long long)B * Hkv;
-    const int roles = two_roles(dtype, DP) ? 2 : 1, tile = tile_of(dtype, DP);
+    const int roles = two_roles(DP) ? 2 : 1, tile = tile_of(dtype, DP);
     pl.rs = 1;
     pl.blocks = heads * ((Tk + 4LL * tile - 1) / (4 * tile));
     if (pl.blocks * roles < 256) {

@@ -283,7 +283,7 @@ template <int DT, int DP, int RS>
 __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP == 64 && RS == 1 ? 3 : 2) void attn_lse_dkv_kernel(Args p) {
     __shared__ __attribute__((aligned(1024))) typename Dkv<DT, DP, RS>::Shared sh;
     const int bid = logical_block(p.xcd_map);
-    if constexpr (two_roles(DT, DP)) {
+    if constexpr (two_roles(DP)) {
         if (bid & 1) dkv_block<DT, DP, RS, 2>(p, bid >> 1, sh);
         else dkv_block<DT, DP, RS, 1>(p, bid >> 1, sh);
     } else dkv_block<DT, DP, RS, 3>(p, bid, sh);
@@ -339,7 +339,7 @@ void launch_bwd(const Args& a, const Ten& dq, const Ten& dk, const Ten& dv, hipS
     x.stripes = stripes_of((long long)a.B * a.Hkv);
     x.splits = pk.splits;
     x.part1 = x.part0 + (long long)pk.splits * a.B * a.Hkv * a.Tk * a.D;
-    const dim3 gk((unsigned)(pk.blocks * pk.splits * (two_roles(DTYPE, DP) ? 2 : 1)));
+    const dim3 gk((unsigned)(pk.blocks * pk.splits * (two_roles(DP) ? 2 : 1)));
     if (pk.rs == 1) hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, 1>), gk, wg, 0, s, x);
     else hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, FEW>), gk, wg, 0, s, x);
     if (pk.splits > 1) {

@@ -156,6 +156,19 @@ SHAPES = [      # b, tq, tk, hq, hkv, d, causal, q_lens, kv_lens, layout
     (1, 513, 513, 1, 1, 128, True, None, None, "legacy"),
     (1, 5, 1030, 8, 1, 16, False, None, None, "separate"),
     (1, 1030, 5, 8, 1, 16, True, None, None, "separate"),
+    # more than 256 blocks: every wave has columns of its own
+    (8, 130, 130, 40, 40, 64, False, None, None, "split"),
+    (5, 100, 133, 60, 20, 32, True, (100, 3, 0, 64, 77), (133, 133, 9, 0, 40), "heads"),
+    (6, 97, 65, 48, 48, 128, True, None, None, "legacy"),
+    (9, 33, 70, 32, 32, 256, False, None, None, "separate"),
+    (9, 80, 40, 32, 32, 96, True, None, None, "separate"),
+    # a few rows over a long axis, both ways: ranges of their own, joined
+    (2, 1, 3001, 8, 2, 64, False, None, None, "separate"),
+    (2, 3, 2500, 6, 2, 128, True, (3, 1), (2500, 700), "heads"),
+    (1, 2, 1500, 2, 2, 256, False, None, None, "separate"),
+    (1, 3001, 3, 4, 2, 64, False, None, None, "separate"),
+    (2, 1500, 40, 2, 1, 128, True, (1500, 900), (40, 40), "separate"),
+    (1, 1400, 1400, 2, 1, 40, True, None, None, "separate"),
 ]
 
 
