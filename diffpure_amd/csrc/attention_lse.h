@@ -400,74 +400,75 @@ inline int stripes_of(long long heads) {
     return s;
 }
 
-// How a launch that keeps queries (forward, dQ) covers the chip of 256 CUs.
-//   packed: heads that share their keys are columns of one block where all their queries fit two tiles (a key is then read once per group).
-//   rs:     waves of a workgroup that share one tile of columns and divide the streamed rows (1: every wave has its own columns).  Sharing makes
-//           four times the workgroups with a quarter of the rows each.
-//   splits: ranges of the streamed rows that workgroups of their own take, joined by a second launch.
+// How a launch covers the chip's 256 CUs.
+//   rs:     waves of a workgroup that share one tile of columns and divide the streamed rows (1: every wave has a tile of its own).  Sharing makes more
+//           workgroups with fewer rows each, but their stages fill the LDS: fewer of them fit a CU.
+//   splits: ranges of the streamed rows that workgroups of their own take; a second launch joins their partial results.
+// The cheapest by this estimate in microseconds: a round of workgroups costs 4 to begin and end and, per stage, the matrix time c of a wave as often as
+// waves share its SIMD - at least twice, the latency of a stage that nothing hides - or the stage's own way into LDS, 0.7 and 60 GB/s per CU; a join costs 5 and the
+// partial results' way to memory and back.
+// A causal mask leaves the blocks half their rows on average, and the longest, begun first, bounds the launch.
+// (One head of 256 channels, 4133 keys and queries, bf16, backward: 145 us, and 409 us without ranges; 1006 queries, 9 keys, fp32: 60 and 120 us.)
+struct Cover {
+    int rs, splits;
+    long long blocks;             // workgroups of one range
+};
+inline Cover cover(int dtype, int DP, long long heads, long long cols, int rows, int times, int roles, double out_bytes, bool causal) {
+    const int tile = tile_of(dtype, DP), srows = dtype == 0 ? 16 : 32, few = DP > 128 ? 2 : 4;
+    const double c = (dtype == 0 ? 1.5 : 0.38 * tile / 32) * DP / 128;
+    static const int cuts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    Cover best{1, 1, 0};
+    double best_t = 1e30;
+    for (int rs = 1; rs <= few; rs += few - 1) {
+        const long long wide = 4 * tile / rs, blocks = heads * ((cols + wide - 1) / wide) * roles;
+        const int resident = rs > 1 ? (DP <= 64 ? 2 : 1) : (DP <= 64 ? 3 : dtype == 0 && DP > 128 ? 1 : 2);
+        const int stages = (rows + rs * srows - 1) / (rs * srows);
+        const double slots = 256.0 * resident;
+        for (int cut : cuts) {
+            if (cut > stages) break;
+            const double wgs = (double)blocks * cut, per = (double)((stages + cut - 1) / cut) * times;
+            const double share = wgs <= 256 ? 1 : wgs >= slots ? resident : (wgs + 255) / 256, copy = 0.7 + 2.0 * rs * srows * DP * (dtype == 0 ? 4 : 2) * share / 60e3;
+            const double turn = (share < 2 ? 2 : share) * c > copy ? (share < 2 ? 2 : share) * c : copy;
+            double t;
+            if (causal) t = 4 + turn * (per / 2 * wgs / slots > per ? per / 2 * wgs / slots : per);
+            else t = (wgs <= 2 * slots ? (double)(long long)((wgs + slots - 1) / slots) : wgs / slots + 0.4) * (4 + turn * per);       // (many rounds run into each other)
+            if (cut > 1) t += 5 + cut * out_bytes * 2 / 4e6;
+            if (t < best_t * 0.999) {
+                best_t = t;
+                best = Cover{rs, cut, blocks};
+            }
+        }
+    }
+    return best;
+}
+
+// The launches that keep queries (forward, dQ).  packed: heads that share their keys are columns of one block where all their queries fit two tiles
+// (a key is then read once per group).
 struct QPlan {
     int packed, rs, splits, split_rows;
     long long blocks;
 };
 inline QPlan q_plan(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int DP) {
-    QPlan pl;                     // a block has 4 / rs tiles of columns
-    const int group = Hq / Hkv, tile = tile_of(dtype, DP), srows = dtype == 0 ? 16 : 32;
-    pl.packed = group > 1 && (long long)group * Tq <= 2 * tile;
-    const long long heads = (long long)B * (pl.packed ? Hkv : Hq), cols = pl.packed ? (long long)group * Tq : Tq;
-    pl.rs = 1;
-    pl.blocks = heads * ((cols + 4 * tile - 1) / (4 * tile));
-    if (cols <= tile || pl.blocks < 256) {
-        pl.rs = DP > 128 ? 2 : 4;
-        const int wide = tile * 4 / pl.rs;
-        pl.blocks = heads * ((cols + wide - 1) / wide);
-    }
-    pl.splits = 1;
-    const int stage = pl.rs * srows;
-    if (pl.blocks < 256) {
-        // one round of workgroups: the stages of two take 2 * 4 * tile rows of 2 * DP elements each, 160 KB hold two workgroups up to 64 channels
-        const long long fill = DP <= 64 ? 512 : 256, want = fill / pl.blocks, most = Tk / (4 * stage);
-        pl.splits = (int)(want < most ? want : most);
-        if (pl.splits < 1) pl.splits = 1;
-        if (pl.splits > 128) pl.splits = 128;
-    }
-    const int stages = (Tk + stage - 1) / stage;
-    pl.split_rows = (stages + pl.splits - 1) / pl.splits * stage;
+    QPlan pl;
+    const int group = Hq / Hkv;
+    pl.packed = group > 1 && (long long)group * Tq <= 2 * tile_of(dtype, DP);
+    const Cover c = cover(dtype, DP, (long long)B * (pl.packed ? Hkv : Hq), pl.packed ? (long long)group * Tq : Tq, Tk, 1, 1, 4.0 * B * Hq * Tq * DP, false);
+    pl.rs = c.rs;
+    pl.blocks = c.blocks;
+    const int stage = pl.rs * (dtype == 0 ? 16 : 32), stages = (Tk + stage - 1) / stage;
+    pl.split_rows = (stages + c.splits - 1) / c.splits * stage;
     pl.splits = (Tk + pl.split_rows - 1) / pl.split_rows;
     return pl;
 }
 
-// The same for the launch that keeps keys (dK, dV).  Its partial sums are as large as 2 * splits results, so it is split for causal launches (whose
-// blocks differ in length) and for those that would leave CUs without a workgroup.
+// The launch that keeps keys (dK, dV).
 // Above 64 channels the two gradients are formed by different workgroups, each of which recomputes the scores: a wave that holds both has 64 accumulators
 // more and leaves no room for a second wave on its SIMD (8191 causal, heads of 128: 1434 us together, 1160 us apart; 128 heads of 256 channels x 256: 78.6 and
 // 76.4 us; heads of 64, where both fit: 182 us together for 32 x 1024 x 8 heads, and 5 products instead of 4 apart).
 constexpr bool two_roles(int DP) { return DP > 64; }
-
-struct KPlan {
-    int rs, splits;
-    long long blocks;
-};
-inline KPlan k_plan(int dtype, int B, int Tq, int Tk, int Hkv, int DP, int causal) {
-    KPlan pl;
-    const long long heads = (long long)B * Hkv;
-    const int roles = two_roles(DP) ? 2 : 1, tile = tile_of(dtype, DP);
-    pl.rs = 1;
-    pl.blocks = heads * ((Tk + 4LL * tile - 1) / (4 * tile));
-    if (pl.blocks * roles < 256) {
-        pl.rs = DP > 128 ? 2 : 4;
-        const int wide = tile * 4 / pl.rs;
-        pl.blocks = heads * ((Tk + wide - 1) / wide);
-    }
-    const int stage = pl.rs * (dtype == 0 ? 16 : 32);
-    pl.splits = 1;
-    const long long fill = causal ? 1024 : 512;
-    if (pl.blocks * roles < (causal ? 1024 : 256)) {
-        const long long want = (fill + pl.blocks * roles - 1) / (pl.blocks * roles), most = Tq / (4 * stage);
-        pl.splits = (int)(want < most ? want : most);
-        if (pl.splits < 1) pl.splits = 1;
-        if (pl.splits > 64) pl.splits = 64;
-    }
-    return pl;
+inline Cover k_plan(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int DP, int causal) {
+    const int roles = two_roles(DP) ? 2 : 1;
+    return cover(dtype, DP, (long long)B * Hkv, Tk, Tq, Hq / Hkv, roles, 8.0 * B * Hkv * Tk * DP, causal != 0);
 }
 
 }  // namespace al

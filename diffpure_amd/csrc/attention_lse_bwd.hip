@@ -335,11 +335,11 @@ void launch_bwd(const Args& a, const Ten& dq, const Ten& dk, const Ten& dv, hipS
     x.w0 = dk;
     x.w1 = dv;
     x.packed = 0;
-    const KPlan pk = k_plan(DTYPE, a.B, a.Tq, a.Tk, a.Hkv, DP, a.causal);
+    const Cover pk = k_plan(DTYPE, a.B, a.Tq, a.Tk, a.Hq, a.Hkv, DP, a.causal);
     x.stripes = stripes_of((long long)a.B * a.Hkv);
     x.splits = pk.splits;
     x.part1 = x.part0 + (long long)pk.splits * a.B * a.Hkv * a.Tk * a.D;
-    const dim3 gk((unsigned)(pk.blocks * pk.splits * (two_roles(DP) ? 2 : 1)));
+    const dim3 gk((unsigned)(pk.blocks * pk.splits));
     if (pk.rs == 1) hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, 1>), gk, wg, 0, s, x);
     else hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, FEW>), gk, wg, 0, s, x);
     if (pk.splits > 1) {
@@ -362,7 +362,7 @@ extern "C" long long dp_attention_lse_bwd_workspace(int dtype, int B, int Tq, in
     if (dtype < 0 || dtype > 2 || B <= 0 || Tq <= 0 || Tk <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return 0;
     const int DP = al::padded_dim(D);
     const al::QPlan pq = al::q_plan(dtype, B, Tq, Tk, Hq, Hkv, DP);
-    const al::KPlan pk = al::k_plan(dtype, B, Tq, Tk, Hkv, DP, 1), pk0 = al::k_plan(dtype, B, Tq, Tk, Hkv, DP, 0);
+    const al::Cover pk = al::k_plan(dtype, B, Tq, Tk, Hq, Hkv, DP, 1), pk0 = al::k_plan(dtype, B, Tq, Tk, Hq, Hkv, DP, 0);
     const long long rows = 2LL * B * Hq * ((Tq + 127LL) / 128 * 128);
     const long long q = pq.splits > 1 ? (long long)pq.splits * B * Hq * Tq * D : 0;
     const int ks = pk.splits > pk0.splits ? pk.splits : pk0.splits;

@@ -153,6 +153,8 @@ SHAPES = [      # b, tq, tk, hq, hkv, d, causal, q_lens, kv_lens, layout
     (3, 64, 200, 2, 2, 96, True, (64, 500, -3), (10, 200, 70), "heads"),      # lengths outside 0 .. T are clamped
     (1, 150, 150, 1, 1, 256, False, None, None, "split"),
     (2, 70, 140, 2, 1, 200, True, None, None, "separate"),
+    (2, 40, 50, 2, 2, 64, True, (40, 7), None, "separate"),
+    (2, 40, 50, 2, 2, 64, False, None, (50, 9), "separate"),
     (1, 513, 513, 1, 1, 128, True, None, None, "legacy"),
     (1, 5, 1030, 8, 1, 16, False, None, None, "separate"),
     (1, 1030, 5, 8, 1, 16, True, None, None, "separate"),
@@ -272,6 +274,30 @@ def test_same_results_twice_on_another_stream_and_in_a_graph():
         torch.cuda.synchronize()
         for _, res in graphs:
             assert all(torch.equal(a, b) for a, b in zip(eager, res)), k_
+
+
+def test_offsets_beyond_32_bits():
+    """tokens 128 KB apart, 40 000 of them: 5 GB between the first and the last; the same results as from dense tensors"""
+    from diffpure_amd import ops
+    t, d = 40000, 64
+    far = torch.empty(t, 65536, device="cuda", dtype=torch.float16)
+    dense = [(0.7 * torch.randn(1, t, 1, d, device="cuda")).half() for _ in range(2)]
+    views = [far[:, i * 1024:i * 1024 + d].view(1, t, 1, d) for i in range(4)]
+    for v, x in zip(views, dense):
+        v.copy_(x)
+    q, _, _, dout = make(torch.float16, 1, 70, 1, 1, 1, d)
+    want = ops.attention_lse(q, *dense)
+    got = ops.attention_lse(q, *views[:2])
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    want = ops.attention_lse_bwd(dout, q, *dense, *want)
+    got = ops.attention_lse_bwd(dout, q, *views[:2], *got, grads=(torch.empty_like(q), views[2], views[3]))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    # and as queries: the streamed operand of dK and dV
+    qs, do = views[0], views[1]
+    k, v = (0.7 * torch.randn(2, 1, 33, 1, d, device="cuda")).half().unbind(0)
+    out, lse = ops.attention_lse(qs, k, v)
+    for a, b in zip(ops.attention_lse_bwd(dense[1], dense[0], k, v, out, lse), ops.attention_lse_bwd(do, qs, k, v, out, lse)):
+        assert torch.equal(a, b)
 
 
 def test_gradients_into_views_and_nothing_beside_them():
