@@ -4,6 +4,13 @@
 // Two kernels, no atomics (results do not depend on the order of workgroups): dQ keeps queries and streams keys (and writes delta and the
 // log2-domain log-sum-exp, +inf where a row has no gradient, for the other), dK / dV keeps keys and streams the queries of every head of its group.
 //
+// Measured on MI355X:
+//   32 x 1024 tokens, 8 heads of 64, fp16    280 us (dQ 137, dK / dV 182 by the profiler's clock, 0.75 PFLOP/s each): bound by the VALU, which forms the
+//                                            exponential in both (16 cycles per wave instruction)
+//   8191 tokens causal, 16 / 4 heads of 128, bf16    1107 us (dQ 380, dK and dV 740: 1.0 and 0.93 PFLOP/s): bound by the matrix instructions of 8 products
+//   128 x 256 tokens, one head of 256, fp16    75 us, of which 30 are kept operands and results
+//   1 x 256 tokens, 16 heads of 64, fp32    20 us: two launches of four stages, latency
+//
 // fp16: the probabilities are formed as 2^6 P (an addend of the exponent) and taken out of the sums again at the end.  dS is rounded to fp16 as
 // operand of its product, and P (dP - delta) of a long row is easily 1e-3 of dout: without the factor it meets fp16's subnormals (below 6e-5) six
 // bits earlier.  |dS| <= P (1 - P) max|dP_i - dP_j|, so 2^6 dS overflows only where the spread of dout v^T along a row passes 4094.

@@ -31,7 +31,8 @@ enum DpTune {
     DP_T_XCD_MAP,          // DP_XCD_MAP (round 6): XCD-aware workgroup maps of the secondary kernels - workgroups are dealt to the 8 XCDs round-robin by
                            // blockIdx, so neighbours in blockIdx order that share cache lines (gn_finalize_cols: four groups per 128-byte record line;
                            // one-pass GroupNorm backward: two 16-channel blocks per line) or stream the same operand (flash attention: the query blocks of
-                           // a head; gemm_strided_h16: the tiles of a batch entry) are re-dealt onto ONE XCD - 0 off; same bits
+                           // a head; gemm_strided_h16: the tiles of a batch entry; the log-sum-exp attention: the blocks of a
+                           // head) are re-dealt onto ONE XCD - 0 off; same bits
     DP_T_COUNT
 };
 

@@ -594,6 +594,10 @@ class GuidedUNet:
         da = self._dconv(dout, n + ".dwproj", r.get("dh2_p", False) == "h1" and "h1", c, 1)
         h16_ok = getattr(self, "_gpool", None) is not None and os.environ.get("DIFFPURE_ATTN_BWD16", "1") != "0"
         qkv = t["qkv"]
+        if ops.attention_recompute_wanted():
+            dqkv = ops.attention_recompute_bwd(qkv.view(b, hh * ww, 3 * c), da.view(b, hh * ww, c), r["heads"], t["layout"])
+            dxn = self._dconv(dqkv.view(b, hh, ww, 3 * c), n + ".dwqkv", r["dh2"], c, 1)
+            return ops.group_norm_bwd(t["x"], self.GN_GROUPS, P[n + ".g"], P[n + ".b"], t["st"], dxn, addend=dout)[0]
         # taped on the fp16 stream: the backward reads q, k, v IN PLACE where all five of its products run on dp_gemm_strided_h16 (NCSN++:
         # T = d = 256); where some shape stays on the fp32-input kernel (64-wide heads: N = 64) the tensor is up-converted once (same values)
         if qkv.dtype == torch.float16 and not (h16_ok and ops.attention_h16_serves(hh * ww, c // r["heads"])):

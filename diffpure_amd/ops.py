@@ -1140,6 +1140,30 @@ def attention_lse_bwd(dout, q, k, v, out, lse, scale=None, causal=False, q_lens=
     return dq, dk, dv
 
 
+def attention_recompute_wanted():
+    """DIFFPURE_ATTN_RECOMPUTE=1: the engines' attention backward (adjoint workloads) runs on attention_lse / attention_lse_bwd: no [B * heads, T, T]
+    tensors (two of 2.1 GB per 32 x 32 layer at B = 64).  Off by default: the low-order bits differ from the product-by-product form."""
+    return os.environ.get("DIFFPURE_ATTN_RECOMPUTE", "0") == "1"
+
+
+def attention_recompute_bwd(qkv, dout, n_heads, layout):
+    """attention_bwd without the probabilities: d qkv [B, T, 3C] (fp32) for dout [B, T, C] fp32, q, k and v read in place from qkv (fp32 or the taped
+    fp16 tensor, whose type the products' operands and the gradient of each token then have)."""
+    if not isinstance(qkv, torch.Tensor) or not qkv.is_cuda or qkv.dim() != 3 or qkv.dtype not in (torch.float32, torch.float16) or not qkv.is_contiguous():
+        raise _lib.DiffpureHipError("attention_recompute_bwd.qkv: expected a contiguous float32 or float16 GPU tensor [B, T, 3C]")
+    b, t, c3 = qkv.shape
+    d = c3 // 3 // n_heads
+    _attn_offsets(c3 // 3, d, layout)                # refuses other layouts
+
+    def heads(x):
+        return x.view(b, t, n_heads, 3, d).unbind(3) if layout == "legacy" else x.view(b, t, 3, n_heads, d).unbind(2)
+    q, k, v = heads(qkv)
+    dqkv = torch.empty_like(qkv)
+    out, lse = attention_lse(q, k, v)
+    attention_lse_bwd(_chk(dout, "attention_recompute_bwd.dout", 3).to(qkv.dtype).view(b, t, n_heads, d), q, k, v, out, lse, grads=heads(dqkv))
+    return dqkv.float()
+
+
 # ---------------------------------------------------------------------------------------------
 # layer norm
 # ---------------------------------------------------------------------------------------------
