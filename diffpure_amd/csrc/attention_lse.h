@@ -426,6 +426,7 @@ inline Cover cover(int dtype, int DP, long long heads, long long cols, int rows,
         const double slots = 256.0 * resident;
         for (int cut : cuts) {
             if (cut > stages) break;
+            if (blocks * cut * 256 >= 1LL << 32) break;             // threads of a grid; the first candidate always fits (dp_attn_lse_common)
             const double wgs = (double)blocks * cut, per = (double)((stages + cut - 1) / cut) * times;
             const double share = wgs <= 256 ? 1 : wgs >= slots ? resident : (wgs + 255) / 256, copy = 0.7 + 2.0 * rs * srows * DP * (dtype == 0 ? 4 : 2) * share / 60e3;
             const double turn = (share < 2 ? 2 : share) * c > copy ? (share < 2 ? 2 : share) * c : copy;
@@ -475,5 +476,6 @@ inline Cover k_plan(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int DP, i
 
 // argument checks shared by the two entry points (attention_lse.hip): message and non-zero / false on a refusal
 bool dp_attn_lse_tensor(const char* fn, const char* name, const void* ptr, const long long* st, int es, int B, int Tn, int H, bool written, al::Ten* t);
+bool dp_attn_lse_apart(const char* fn, const char* name, const al::Ten& w, int wt, int wh, const char* other, const al::Ten& r, int rt, int rh, int B, long long row);
 int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq,
                        int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, al::Args* a);

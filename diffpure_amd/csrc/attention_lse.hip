@@ -240,6 +240,21 @@ bool dp_attn_lse_tensor(const char* fn, const char* name, const void* ptr, const
     return true;
 }
 
+// a written tensor against a read one: their bytes from first to last must lie apart, or their tokens must be different columns of rows at one pitch
+bool dp_attn_lse_apart(const char* fn, const char* name, const al::Ten& w, int wt, int wh, const char* other, const al::Ten& r, int rt, int rh, int B, long long row) {
+    const long long ww = (wh - 1LL) * w.h + row, rw = (rh - 1LL) * r.h + row;                  // a token's bytes, its heads apart or side by side
+    const long long wend = (B - 1LL) * w.b + (wt - 1LL) * w.t + ww, rend = (B - 1LL) * r.b + (rt - 1LL) * r.t + rw, at = (intptr_t)r.p - (intptr_t)w.p;
+    if (at >= wend || -at >= rend) return true;
+    const bool one = wt == 1 && rt == 1;                                                       // single tokens: a row of each sample
+    const long long pitch = one ? w.b : w.t;
+    if (pitch > 0 && (one ? r.b : r.t) == pitch && (one || (w.b % pitch == 0 && r.b % pitch == 0))) {
+        const long long col = (at % pitch + pitch) % pitch;                                    // where r's token begins in w's row
+        if (col >= ww && col + rw <= pitch) return true;
+    }
+    dp_set_error("%s: %s overlaps %s", fn, name, other);
+    return false;
+}
+
 int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq,
                        int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, al::Args* a) {
     DP_REQUIRE(strides, "%s: strides missing", fn);
@@ -283,6 +298,10 @@ extern "C" int dp_attention_lse(const void* q, const void* k, const void* v, con
     if (!dp_attn_lse_tensor(fn, "out", out, strides + 9, dtype == 0 ? 4 : 2, B, Tq, Hq, true, &a.w0)) return 1;
     const long long need = dp_attention_lse_workspace(dtype, B, Tq, Tk, Hq, Hkv, D);
     DP_REQUIRE(need == 0 || (work && dp_aligned16(work) && work_bytes >= need), "%s: workspace of %lld bytes needed (got %lld)", fn, need, work_bytes);
+    const long long row = (long long)D * (dtype == 0 ? 4 : 2);
+    if (!dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "q", a.q, Tq, Hq, B, row) || !dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "k", a.k, Tk, Hkv, B, row) ||
+        !dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "v", a.v, Tk, Hkv, B, row))
+        return 1;
     a.lse = lse;
     a.part0 = static_cast<float*>(work);
     a.part_lse = need ? a.part0 + need / 4 / (D + 1) * D : nullptr;

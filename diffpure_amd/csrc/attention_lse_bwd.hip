@@ -392,6 +392,12 @@ extern "C" int dp_attention_lse_bwd(const void* dout, const void* q, const void*
         return 1;
     const long long need = dp_attention_lse_bwd_workspace(dtype, B, Tq, Tk, Hq, Hkv, D);
     DP_REQUIRE(work && dp_aligned16(work) && work_bytes >= need, "%s: workspace of %lld bytes needed (got %lld)", fn, need, work_bytes);
+    const struct { const char* name; al::Ten t; int tokens, heads; } wr[3] = {{"dq", tq, Tq, Hq}, {"dk", tk, Tk, Hkv}, {"dv", tv, Tk, Hkv}},
+        rd[5] = {{"q", a.q, Tq, Hq}, {"k", a.k, Tk, Hkv}, {"v", a.v, Tk, Hkv}, {"out", a.o, Tq, Hq}, {"dout", a.dout, Tq, Hq}};
+    for (const auto& w : wr)
+        for (const auto& r : rd)
+            if (!dp_attn_lse_apart(fn, w.name, w.t, w.tokens, w.heads, r.name, r.t, r.tokens, r.heads, B, (long long)D * es)) return 1;
+    DP_REQUIRE(dq != dk && dq != dv && dk != dv, "%s: dq, dk and dv begin at one address", fn);        // (views of one tensor interleave)
     a.lse = const_cast<float*>(lse);
     a.rows = static_cast<float*>(work);
     a.part0 = a.rows + 2LL * B * Hq * a.Tqp;

@@ -1102,7 +1102,7 @@ def _attn_lse_args(fn, q, k, v, scale, q_lens, kv_lens):
 def attention_lse(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
     """softmax(scale q k^T + mask) v and the log-sum-exp of its rows: q [B, Tq, Hq, D], k, v [B, Tk, Hkv, D] -> out [B, Tq, Hq, D] (contiguous),
     lse [B, Hq, Tq] fp32.  fp32 / fp16 / bf16, any strides that are multiples of 16 bytes (views of one qkv tensor in either head order), any token
-    counts, D a multiple of 8 up to 256, Hq a multiple of Hkv (query heads h * Hq / Hkv ... share key head h); scale None = 1 / sqrt(D).
+    counts from 1, D a multiple of 8 up to 256, Hq a multiple of Hkv (query heads h * Hq / Hkv ... share key head h); scale None = 1 / sqrt(D).
     q_lens / kv_lens: int32 [B], valid tokens per sample; causal: the last valid row sees every valid key, each row before it one fewer.
     Rows that see nothing give 0 and -inf.  The statistics are what attention_lse_bwd recomputes the probabilities from (csrc/attention_lse.hip)."""
     st, args = _attn_lse_args("attention_lse", q, k, v, scale, q_lens, kv_lens)
@@ -1120,7 +1120,7 @@ def attention_lse(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
 def attention_lse_bwd(dout, q, k, v, out, lse, scale=None, causal=False, q_lens=None, kv_lens=None, grads=None):
     """Gradients (dq, dk, dv) of attention_lse's `out` for the cotangent dout, given its results and the arguments of the forward call.  No [Tq, Tk] tensor
     and no atomics; a key head's gradient is the sum over the query heads that share it.  grads=(dq, dk, dv): written into these tensors (of
-    q's type; views of one dqkv tensor, say) instead of new contiguous ones."""
+    q's type; views of one dqkv tensor, say, that lies apart from every input) instead of new contiguous ones."""
     st, args = _attn_lse_args("attention_lse_bwd", q, k, v, scale, q_lens, kv_lens)
     b, tq, hq, d = q.shape
     st += _heads(out, "attention_lse_bwd.out", q, q.shape) + _heads(dout, "attention_lse_bwd.dout", q, q.shape)

@@ -46,6 +46,33 @@ def test_attention_lse_bwd_refuses(kw, what):
     assert what in lib().dp_last_error(), lib().dp_last_error()
 
 
+@pytest.mark.parametrize("off,what", [(0, b"out overlaps q"), (2 * 8 * 2 * 16 * 2 - 16, b"out overlaps q"), (-16, b"out overlaps q"), (1 << 20, b"out overlaps k"), (2 << 20, b"out overlaps v")])
+def test_attention_lse_refuses_outputs_on_inputs(off, what):
+    q = 1 << 24
+    assert attn_fwd(q=q, k=q + (1 << 20), v=q + (2 << 20), out=q + off) != 0
+    assert what in lib().dp_last_error(), lib().dp_last_error()
+
+
+def test_attention_lse_columns_of_one_row_are_apart():
+    """q and out as columns of rows of 128: 32 columns to the right they pass that check (and are refused for the next tensor), nearer or beyond the row's end not"""
+    for tq, b in ((1, 2), (6, 1), (6, 2)):
+        st = [128 * tq, 128, 16, 256, 32, 16, 256, 32, 16, 128 * tq, 128, 16]
+        for col, what in ((0, b"q"), (16, b"q"), (24, b"q"), (112, b"q"), (32, b"k"), (96, b"k")):
+            out = (1 << 24) + 2 * col
+            assert attn_fwd(q=1 << 24, k=out, v=1 << 27, out=out, b=b, tq=tq, strides=st) != 0
+            assert b"out overlaps " + what in lib().dp_last_error(), (tq, b, col, lib().dp_last_error())
+
+
+@pytest.mark.parametrize("grads,what", [((0, 10, 11), b"dq overlaps q"), ((10, 0, 11), b"dk overlaps q"), ((10, 11, 2), b"dv overlaps v"), ((10, 4, 11), b"dk overlaps dout"),
+                                        ((3, 10, 11), b"dq overlaps out"), ((10, 10, 11), b"one address"), ((10, 11, 11), b"one address"), ((11, 10, 11), b"one address")])
+def test_attention_lse_bwd_refuses_gradients_on_inputs(grads, what):
+    at = lambda i: (1 << 24) + (i << 20)                  # q, k, v, out, dout lie at 0 .. 4, lse at 5, the workspace at 6
+    st = (C.c_longlong * 24)(*[256, 32, 16] * 8)
+    assert lib().dp_attention_lse_bwd(at(4), at(0), at(1), at(2), at(3), at(5), C.addressof(st), 1, 2, 8, 8, 2, 2, 16, None, None, 0.25, 0, *map(at, grads), at(6), 1 << 30,
+                                      None) != 0
+    assert what in lib().dp_last_error(), lib().dp_last_error()
+
+
 def test_attention_workspace_sizes():
     fwd, bwd = lib().dp_attention_lse_workspace, lib().dp_attention_lse_bwd_workspace
     for ws in (fwd, bwd):
