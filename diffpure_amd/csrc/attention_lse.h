@@ -224,6 +224,10 @@ __device__ __forceinline__ int logical_block(int xcd_map) {
     return bid;
 }
 
+// keys that query `tok` of a sample with n queries and m keys sees: lengths and the causal diagonal alone decide which rows are empty (a sum of
+// probabilities does not: it is NaN where a score is, and 0 where every score is -inf)
+__device__ __forceinline__ int keys_seen(int tok, int n, int m, int causal) { return tok >= n ? 0 : causal ? min(m, tok + m - n + 1) : m; }
+
 __device__ __forceinline__ int clamp_len(const int* lens, int b, int t) {
     if (!lens) return t;
     const int n = lens[b];

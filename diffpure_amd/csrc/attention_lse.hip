@@ -124,7 +124,8 @@ __global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_fwd_kernel(Args p) {
 #pragma unroll
         for (int w = 0; w < RS; ++w) sum += ml[1][wave - rw + w][cl] * __builtin_amdgcn_exp2f(ml[0][wave - rw + w][cl] * c - tc);
     }
-    const bool some = tok < n && sum > 0.f, out = col < kept.cols;
+    // a range in which a row meets no key (or scores of -inf only) has weight 0 in the join; a row that sees keys and sums to 0 in all is 0 / 0
+    const bool some = keys_seen(tok, n, m, p.causal) > 0 && (p.splits == 1 || sum != 0.f), out = col < kept.cols;
     const float inv = some ? 1.f / sum : 0.f, lse = some ? top * fabsf(p.scale) + logf(sum) : -INFINITY;
     const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
     char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head * p.w0.h + tok * p.w0.t;
@@ -160,7 +161,8 @@ __global__ __launch_bounds__(256) void attn_lse_join_kernel(Args p) {
     const Kept kept(p, z);
     int h, t;
     kept.col(p, (int)(kr - (long long)z * cols), h, t);
-    // eight loads under way at a time (ranges behind the last one repeat it with weight 0)
+    const bool some = keys_seen(t, clamp_len(p.q_lens, kept.b, p.Tq), clamp_len(p.kv_lens, kept.b, p.Tk), p.causal) > 0;
+    // eight loads under way at a time (ranges behind the last one repeat it with weight 0); a range that is NaN is not the largest, but its weight is NaN
     float top = -INFINITY, sum = 0.f;
     for (int s0 = 0; s0 < p.splits; s0 += 8) {
         float l[8];
@@ -170,7 +172,8 @@ __global__ __launch_bounds__(256) void attn_lse_join_kernel(Args p) {
         for (int i = 0; i < 8; ++i) top = fmaxf(top, l[i]);
     }
     f32x4 v = {};
-    if (top > -INFINITY) {
+    if (top == -INFINITY) top = 0.f;
+    if (some) {
         for (int s0 = 0; s0 < p.splits; s0 += 8) {
             float l[8];
             f32x4 x[8];
@@ -190,7 +193,7 @@ __global__ __launch_bounds__(256) void attn_lse_join_kernel(Args p) {
         v *= 1.f / sum;
     }
     st4<DT>(const_cast<char*>(p.w0.p) + kept.b * p.w0.b + h * p.w0.h + t * p.w0.t, d, v);
-    if (d == 0) p.lse[((long long)kept.b * p.Hq + h) * p.Tq + t] = top > -INFINITY ? top + logf(sum) : -INFINITY;
+    if (d == 0) p.lse[((long long)kept.b * p.Hq + h) * p.Tq + t] = some ? top + logf(sum) : -INFINITY;
 }
 
 template <int DTYPE, int DP>
