@@ -1,6 +1,7 @@
 // Backward pass of attention_lse.hip.  The probabilities are recomputed from the log-sum-exp, tile by tile:
 //     P = exp(scale q k^T - lse)     delta_i = sum_d dout_id out_id     dP = dout v^T     dS = P (dP - delta)
 //     dV = P^T dout                  dQ = scale dS K                    dK = scale dS^T Q        (key heads: summed over the heads that share them)
+// Rows without a key have P = 0 (a log-sum-exp of +inf); a row whose log-sum-exp is NaN has NaN gradients.
 // Two kernels, no atomics (results do not depend on the order of workgroups): dQ keeps queries and streams keys (and writes delta and the
 // log2-domain log-sum-exp, +inf where a row has no gradient, for the other), dK / dV keeps keys and streams the queries of every head of its group.
 //
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     delta = col_sum<T::TILE>(delta);
     const long long zh = (long long)b * p.Hq + head;
     const float lse = p.lse[zh * p.Tq + krow];
-    const bool some = tok < n && lse > -INFINITY;
+    const bool some = keys_seen(tok, n, m, p.causal) > 0;       // (not by lse: a NaN must reach the gradients)
     const float l2 = some ? lse * LOG2E - (float)T::PSHIFT : INFINITY;
     if (!some) delta = 0.f;
     if (g == 0 && rw == 0 && split == 0 && col < kept.cols) {
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     const bool out = col < kept.cols;
     const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
     char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head * p.w0.h + tok * p.w0.t;
-    const float mul = tok < n ? p.scale / (float)(1 << T::PSHIFT) : 0.f;
+    const float mul = some ? p.scale / (float)(1 << T::PSHIFT) : 0.f;
     if (RS == 1 && p.splits == 1) {
         __syncthreads();
         const int first = c0 + wave * T::TILE;

@@ -418,7 +418,8 @@ int dp_resize_affine_bwd(const float* dy, int B, int C, int Ho, int Wo, int out_
  *     hold anything (NaN too): their out and gradients are written as 0, their lse as -inf.
  *   causal != 0: row i of a sample sees keys 0 .. i + (keys - rows) of it (the last row sees every key).  Inside the lengths values must be finite for the mask to
  *     hide them.  A row that sees no key (by the lengths and causal alone) has out 0, lse -inf, and contributes no gradient.  A row that sees a score of NaN or
- *     +inf (finite inputs may overflow to it) has NaN in out and lse; one whose scores are all -inf has out NaN, lse -inf.
+ *     +inf (finite inputs may overflow to it) has NaN in out and lse; one whose scores are all -inf has out NaN, lse -inf.  The backward pass carries it on: dq of a row whose lse is NaN,
+ *     and dk, dv of the keys it sees, are NaN.
  *   scale: finite, not 0.
  *   work: dp_attention_lse_workspace / dp_attention_lse_bwd_workspace bytes, 16-byte aligned, free again when the call's work on `stream` is done (the
  *     forward pass needs none - 0 - where the queries fill the chip).  The outputs may not overlap any input (refused; columns of

@@ -107,3 +107,52 @@ def test_rows_without_a_key_stay_zero():
                 assert (out[i, none] == 0).all() and (lse[i][:, none] == -math.inf).all()
             met = ((torch.arange(tq) < ql[0]) & (torch.arange(tq) + kl[0] - ql[0] >= 3)).cuda()
             assert torch.isnan(out[0, met, :2]).all() and torch.isfinite(out[0, :, 2:]).all()
+
+
+BACK = FORMS + [(1, 3001, 3, 4, 2, 64, False), (2, 1500, 40, 2, 1, 128, True), (9, 33, 70, 32, 32, 256, False)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("form", BACK, ids=FORM_IDS + ["few_keys", "few_keys_causal", "wide_heads"])
+@pytest.mark.parametrize("what", ["statistics", "query"])
+def test_gradients_of_a_row_that_is_nan(dtype, form, what):
+    """One row of one head is NaN - its log-sum-exp alone (scores, out and dout finite), or as the forward pass leaves it for a NaN query: its dq, and dk and dv of every
+    key it sees, are NaN, not the 0 of a row without keys.  Other heads of the sample and other samples do not notice."""
+    from diffpure_amd import ops
+    b, tq, tk, hq, hkv, d, causal = form
+    q, k, v, dout = make(dtype, b, tq, tk, hq, hkv, d, seed=29)
+    ref, group = Ref(q, k, v, None, causal, None, None), hq // hkv
+    i, h, s = tq - 1, hq - 1, b - 1                                  # the last row of the last head sees a key under a diagonal too
+    if what == "query":
+        q[s, i, h, 5] = float("nan")
+    out, lse = ops.attention_lse(q, k, v, None, causal)
+    if what == "statistics":
+        lse[s, h, i] = float("nan")
+    dq, dk, dv = ops.attention_lse_bwd(dout, q, k, v, out, lse, None, causal)
+    assert torch.isnan(dq[s, i, h]).all(), "dq of the row"
+    at = torch.arange(tk)[seen(b, tq, tk, causal)[0, i]].cuda()
+    assert torch.isnan(dk[s, at, hkv - 1]).all() and torch.isnan(dv[s, at, hkv - 1]).all(), "dk and dv of the keys that it sees"
+    (rq, rk, rv), (uq, uk, uv) = ref.bwd(dout, None)
+    fq, fk = torch.ones(b, hq, dtype=torch.bool), torch.ones(b, hkv, dtype=torch.bool)
+    fq[s, (hkv - 1) * group:] = False
+    fk[s, hkv - 1] = False
+    for name, g, r, t, f in (("dq", dq, rq, uq, fq), ("dk", dk, rk, uk, fk), ("dv", dv, rv, uv, fk)):
+        g, r, t = (x.detach().double().cpu().transpose(1, 2)[f] for x in (g, r, t))
+        close(g, r, t, name)
+
+
+def test_gradients_of_rows_without_a_key_stay_zero():
+    """by the lengths or the diagonal: dq 0 and nothing added to dk and dv, whatever the log-sum-exp that is handed in says"""
+    from diffpure_amd import ops
+    for dtype in TYPES:
+        q, k, v, dout = make(dtype, 3, 90, 40, 4, 2, 64, seed=31)
+        ql, kl = lens_of(90, 50, 7), lens_of(40, 0, 12)
+        ref = Ref(q, k, v, None, True, ql, kl)
+        out, lse = ops.attention_lse(q, k, v, None, True, ql, kl)
+        assert (lse == -math.inf).any()
+        for fill in (-math.inf, math.inf, 3.0, float("nan")):
+            given = torch.where(lse == -math.inf, torch.full_like(lse, fill), lse)
+            grads = ops.attention_lse_bwd(dout, q, k, v, out, given, None, True, ql, kl)
+            res, tol = ref.bwd(dout, ql)
+            for name, g, r, t in zip(("dq", "dk", "dv"), grads, res, tol):
+                close(g, r, t, name)
