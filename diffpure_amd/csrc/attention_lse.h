@@ -350,6 +350,8 @@ struct Args {
     Ten w0, w1;                   // what the kernel writes: out (forward), dq, or dk and dv
     float* lse;                   // [B, Hq, Tq]
     float* rows;                  // backward: [2][B, Hq, Tqp] log2-domain log-sum-exp (+inf: no such row) and -delta
+    int *lost_q, *lost_k;         // backward, fp16: did a wave of the dQ / dK launch lose an element to infinity?  Those of a key head side by side, lost_qn / lost_kn
+    int lost_qn, lost_kn;
     float *part0, *part1;         // split launches: partial results, [split][kept row][D] (the order of kept rows: see Kept)
     float* part_lse;              // forward: [split][kept row]
     const int *q_lens, *kv_lens;

@@ -14,22 +14,32 @@
 //
 // fp16: the probabilities are formed as 2^6 P (an addend of the exponent) and taken out of the sums again at the end.  dS is rounded to fp16 as
 // operand of its product, and P (dP - delta) of a long row is easily 1e-3 of dout: without the factor it meets fp16's subnormals (below 6e-5) six
-// bits earlier.  |dS| <= P (1 - P) max|dP_i - dP_j|, so 2^6 dS overflows only where the spread of dout v^T along a row passes 4094.
+// bits earlier.  Large cotangents (a scaled loss) bring 2^6 dS, or dS itself, beyond 65504.  Such an element is infinite, and so, or NaN, is every sum that it
+// enters: a wave that finds one says so, and a last launch (attn_lse_again: 4 us where there is none) forms those columns anew, with 2^-6, 2^-18 and 2^-30 dS
+// (|dS| < 2^39) until they are finite - or lost because the input is.  In tiles of the first two launches a test for it costs more (dQ of 32 x 1024 tokens x 8 heads:
+// 122 us, 128 with a running maximum of |dS|, 140 with a second loop in the same kernel, whose registers the first then lacks).
 #include "attention_lse.h"
 
 namespace {
 using namespace al;
 
-// dQ.  Workgroups, stages and RS as in the forward kernel.
-template <int DT, int DP, int RS>
-__global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP == 64 && RS == 1 ? 3 : 2) void attn_lse_dq_kernel(Args p) {
+template <int DT, int DP, int RS> struct Dq {
+    using St = Stream<DP * Tr<DT>::ES, Tr<DT>::ES, RS * Tr<DT>::ROWS, 4>;
+    struct Shared { char stage[2 * St::STAGE]; };
+};
+// an element of a written tensor that is infinite or NaN
+__device__ __forceinline__ bool not_finite16(const char* x) { return (*reinterpret_cast<const unsigned short*>(x) & 0x7c00) == 0x7c00; }
+
+// dQ.  Workgroups, stages and RS as in the forward kernel.  AGAIN: the queries among the workgroup's whose dq (all of a query's channels, or none) is not finite.
+template <int DT, int DP, int RS, bool AGAIN>
+__device__ __forceinline__ void dq_block(const Args& p, int bid0, typename Dq<DT, DP, RS>::Shared& sh) {
     using T = Tr<DT>;
     constexpr int NW = 4, BM = RS * T::ROWS, RB = DP * T::ES, KS = DP / T::KSTEP, ND = DP / T::TILE, NKK = T::ROWS / T::KROWS, COLS = NW / RS * T::TILE;
-    using St = Stream<RB, T::ES, BM, NW>;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * St::STAGE];
+    using St = typename Dq<DT, DP, RS>::St;
+    char* smem = sh.stage;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rw = wave % RS, cl = lane & (T::TILE - 1), g = lane / T::TILE;
-    const int bid0 = logical_block(p.xcd_map), split = bid0 % p.splits, bid = bid0 / p.splits;
+    const int split = bid0 % p.splits, bid = bid0 / p.splits;
     const int cols0 = p.packed ? p.Hq / p.Hkv * p.Tq : p.Tq, nblk = (cols0 + COLS - 1) / COLS;
     const int z = bid / nblk, blk = block_of(p, bid - z * nblk, nblk, true);
     if (z >= p.B * (p.packed ? p.Hkv : p.Hq)) return;
@@ -44,6 +54,11 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     typename T::Frag qf[KS], df[KS];
     int head, tok;
     kept.col(p, col < kept.cols ? col : kept.cols - 1, head, tok);
+    bool lost = false;
+    if constexpr (AGAIN) {
+        lost = not_finite16(p.w0.p + b * p.w0.b + head * p.w0.h + tok * p.w0.t);
+        if (!__syncthreads_or(lost)) return;
+    }
     const int krow = tok < n ? tok : (n > 0 ? n - 1 : 0);
     ld_kept<DT, KS>(qf, p.q.p + b * p.q.b + head * p.q.h + krow * p.q.t, row_slots, g);
     ld_kept<DT, KS>(df, p.dout.p + b * p.dout.b + head * p.dout.h + krow * p.dout.t, row_slots, g);
@@ -60,13 +75,13 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     const long long zh = (long long)b * p.Hq + head;
     const float lse = p.lse[zh * p.Tq + krow];
     const bool some = keys_seen(tok, n, m, p.causal) > 0;       // (not by lse: a NaN must reach the gradients)
-    const float l2 = some ? lse * LOG2E - (float)T::PSHIFT : INFINITY;
+    float l2 = some ? lse * LOG2E - (float)T::PSHIFT : INFINITY;
     if (!some) delta = 0.f;
-    if (g == 0 && rw == 0 && split == 0 && col < kept.cols) {
+    if (!AGAIN && g == 0 && rw == 0 && split == 0 && col < kept.cols) {
         p.rows[zh * p.Tqp + tok] = l2;
         p.rows[half + zh * p.Tqp + tok] = -delta;
     }
-    if (blk == nblk - 1 && split == 0) {          // the rows that round Tq up: no such query
+    if (!AGAIN && blk == nblk - 1 && split == 0) {          // the rows that round Tq up: no such query
         const int pad = p.Tqp - p.Tq, heads = p.packed ? p.Hq / p.Hkv : 1;
         for (int i = threadIdx.x; i < pad * heads; i += 256) {
             const long long at = ((long long)b * p.Hq + kept.h0 + i / pad) * p.Tqp + p.Tq + i % pad;
@@ -88,8 +103,8 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     open = begin + max(open - begin, 0) / BM * BM;
     St st;
     st.init(p.k.p + b * p.k.b + kept.hk * p.k.h, p.k.t, p.v.p + b * p.v.b + kept.hk * p.v.h, p.v.t, row_slots, wave, lane);
-    if (begin < end) st.issue(smem, begin, m, 0, 0);
-    int cur = 0;
+    if (!AGAIN && begin < end) st.issue(smem, begin, m, 0, 0);
+    int cur = 0, low = 0;                         // 2^(PSHIFT - low) dS is carried
     auto body = [&](int r0, auto masked) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -119,16 +134,43 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
         }
         settle();
     };
-    int r0 = begin;
-    for (; r0 < open; r0 += BM) body(r0, no{});
-    for (; r0 < end; r0 += BM) body(r0, yes{});
+    auto sweep = [&]() {
+        int r0 = begin;
+        for (; r0 < open; r0 += BM) body(r0, no{});
+        for (; r0 < end; r0 += BM) body(r0, yes{});
+    };
+    if constexpr (AGAIN) {
+        bool still = lost;
+        do {
+            if (still) {
+                l2 += 12.f;
+                low += 12;
+            }
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) dq[dt] = typename T::Acc{};
+            if (begin < end) st.issue(smem + cur * St::STAGE, begin, m, 0, 0);
+            sweep();
+            still = !(fabsf(dq[0][0]) < INFINITY);
+        } while (__syncthreads_or(still && low < 36));
+    } else {
+        sweep();
+        if constexpr (T::PSHIFT > 0) {
+            const bool any = __any(!(fabsf(dq[0][0]) < INFINITY));
+            if (lane == 0) p.lost_q[(((long long)z * nblk + blk) * p.splits + split) * NW + wave] = any;
+        }
+    }
 
     if constexpr (RS > 1) __syncthreads();
     const bool out = col < kept.cols;
     const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
     char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head * p.w0.h + tok * p.w0.t;
-    const float mul = some ? p.scale / (float)(1 << T::PSHIFT) : 0.f;
-    if (RS == 1 && p.splits == 1) {
+    const float mul = some ? (AGAIN ? ldexpf(p.scale, low - T::PSHIFT) : p.scale / (float)(1 << T::PSHIFT)) : 0.f;
+    if constexpr (AGAIN) {
+        join_units<DT, ND, 1>(dq, mul, smem, wave, 0, lane, [&](int u, f32x4 v) {
+            const int d = Units<DT, ND>::d(u, g);
+            if (out && lost && d < p.D) st4<DT>(row, d, v);
+        });
+    } else if (RS == 1 && p.splits == 1) {
         __syncthreads();
         const int first = c0 + wave * T::TILE;
         store_cols<DT, ND, RB>(dq, mul, smem + wave * T::TILE * RB, lane, row_slots, [&](int i) -> char* {
@@ -144,7 +186,14 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     });
 }
 
-// dK and dV: keys are kept, the queries of every head of the group stream by, one head after the other.  WHAT: 1 dK, 2 dV, 3 both.
+template <int DT, int DP, int RS>
+__global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP == 64 && RS == 1 ? 3 : 2) void attn_lse_dq_kernel(Args p) {
+    __shared__ __attribute__((aligned(1024))) typename Dq<DT, DP, RS>::Shared sh;
+    dq_block<DT, DP, RS, false>(p, logical_block(p.xcd_map), sh);
+}
+
+// dK and dV: keys are kept, the queries of every head of the group stream by, one head after the other.  WHAT: 1 dK, 2 dV, 3 both.  AGAIN: the dK among the workgroup's
+// that are not finite; they take their exponents' addends lowered, the same for all, and a key's dK is that of the first pass in which it is finite.
 template <int DT, int DP, int RS> struct Dkv {
     static constexpr int NW = 4, BM = RS * Tr<DT>::ROWS, RB = DP * Tr<DT>::ES, STATS = 2 * BM < 64 ? 64 : 2 * BM;
     using St = Stream<RB, Tr<DT>::ES, BM, NW>;
@@ -153,7 +202,7 @@ template <int DT, int DP, int RS> struct Dkv {
         float rows[2][STATS];             // stage: BM log-sum-exps, then BM -delta of the streamed queries (copied by whole waves)
     };
 };
-template <int DT, int DP, int RS, int WHAT>
+template <int DT, int DP, int RS, int WHAT, bool AGAIN>
 __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<DT, DP, RS>::Shared& sh) {
     using T = Tr<DT>;
     using K = Dkv<DT, DP, RS>;
@@ -174,6 +223,11 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
     const int row_slots = p.D * T::ES / 16;
     const float c = p.scale * LOG2E;
 
+    bool lost = false;
+    if constexpr (AGAIN) {
+        lost = not_finite16(p.w1.p + b * p.w1.b + hk * p.w1.h + (col < p.Tk ? col : p.Tk - 1) * p.w1.t);
+        if (!__syncthreads_or(lost)) return;
+    }
     typename T::Frag kf[KS], vf[DK ? KS : 1];
     typename T::Acc dk[DK ? ND : 1], dv[DV ? ND : 1];
     const int krow = col < m ? col : (m > 0 ? m - 1 : 0);
@@ -207,10 +261,14 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
     // Rows are taken from the last one down: a causal mask lets the blocks of a head begin at different rows but end at the same one, and the blocks that run
     // at a time share what they stream (in L2) only while they stand at the same row.
     const int last = begin + (end - begin - 1) / BM * BM;
-    int cur = 0;
+    int cur = 0, low = 0;                         // 2^(PSHIFT - low) dS is carried
     auto body = [&](int head, int r0, auto masked) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+        if constexpr (AGAIN) {
+            if (tid < BM) sh.rows[cur][tid] += (float)low;
+            __syncthreads();
+        }
         const bool wrap = r0 == begin;
         if (!wrap || head + 1 < group) issue(cur ^ 1, wrap ? head + 1 : head, wrap ? last : r0 - BM);
         const char *Qs = smem + cur * St::STAGE + rw * T::ROWS * RB, *Ds = Qs + St::TILE_BYTES;
@@ -257,13 +315,38 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
         }
         settle();
     };
-    if (begin < end) {
-        issue(0, 0, last);
+    auto sweep = [&]() {
         for (int head = 0; head < group; ++head) {
             int r0 = last;
             for (; r0 >= open; r0 -= BM) body(head, r0, no{});
             for (; r0 >= begin; r0 -= BM) body(head, r0, yes{});
         }
+    };
+    if constexpr (AGAIN) {
+        if (begin >= end) return;
+        char* row = const_cast<char*>(p.w1.p) + b * p.w1.b + hk * p.w1.h + (col < p.Tk ? col : p.Tk - 1) * p.w1.t;
+        do {
+            low += 12;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) dk[dt] = typename T::Acc{};
+            issue(cur, 0, last);
+            sweep();
+            const bool found = lost && fabsf(dk[0][0]) < INFINITY;
+            join_units<DT, ND, 1>(dk, col < m ? ldexpf(p.scale, low - T::PSHIFT) : 0.f, smem, wave, 0, lane, [&](int u, f32x4 v) {
+                const int d = Units<DT, ND>::d(u, g);
+                if (found && col < p.Tk && d < p.D) st4<DT>(row, d, v);
+            });
+            lost = lost && !found;
+        } while (__syncthreads_or(lost && low < 36));
+        return;
+    }
+    if (begin < end) {
+        issue(0, 0, last);
+        sweep();
+    }
+    if constexpr (T::PSHIFT > 0 && DK) {
+        const bool any = __any(!(fabsf(dk[0][0]) < INFINITY));
+        if (lane == 0) p.lost_k[(long long)bid0 * NW + wave] = any;
     }
 
     const bool out = col < p.Tk;
@@ -292,9 +375,32 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     __shared__ __attribute__((aligned(1024))) typename Dkv<DT, DP, RS>::Shared sh;
     const int bid = logical_block(p.xcd_map);
     if constexpr (two_roles(DP)) {
-        if (bid & 1) dkv_block<DT, DP, RS, 2>(p, bid >> 1, sh);
-        else dkv_block<DT, DP, RS, 1>(p, bid >> 1, sh);
-    } else dkv_block<DT, DP, RS, 3>(p, bid, sh);
+        if (bid & 1) dkv_block<DT, DP, RS, 2, false>(p, bid >> 1, sh);
+        else dkv_block<DT, DP, RS, 1, false>(p, bid >> 1, sh);
+    } else dkv_block<DT, DP, RS, 3, false>(p, bid, sh);
+}
+
+// fp16: what the launches before lost, first the queries' blocks, then the keys'.  Nothing is shared with another workgroup, and nothing cut into ranges.  One workgroup
+// per CU takes `per` blocks, and leaves if nothing was lost in the key heads that they belong to.
+template <int DT, int DP>
+__global__ __launch_bounds__(256) AL_WAVES(DP > 64 ? 1 : 2) void attn_lse_again_kernel(Args p, int q_blocks, int blocks, int per) {
+    __shared__ __attribute__((aligned(1024))) union {
+        typename Dq<DT, DP, 1>::Shared q;
+        typename Dkv<DT, DP, 1>::Shared k;
+    } sh;
+    constexpr int COLS = 4 * Tr<DT>::TILE;
+    const int begin = blockIdx.x * per, end = min(begin + per, blocks), q_end = min(end, q_blocks), k_begin = max(begin, q_blocks);
+    const int qn = (p.Tq + COLS - 1) / COLS * (p.Hq / p.Hkv), kn = (p.Tk + COLS - 1) / COLS;       // blocks of a key head
+    int any = 0;
+    auto look = [&](const int* lost, int n, int z0, int z1) {
+        for (long long i = (long long)z0 * n + threadIdx.x; i < (z1 + 1LL) * n; i += 256) any |= lost[i];
+    };
+    if (begin < q_end) look(p.lost_q, p.lost_qn, begin / qn, (q_end - 1) / qn);
+    if (k_begin < end) look(p.lost_k, p.lost_kn, (k_begin - q_blocks) / kn, (end - 1 - q_blocks) / kn);
+    if (!__syncthreads_or(any)) return;
+    for (int i = begin; i < q_end; ++i) dq_block<DT, DP, 1, true>(p, i, sh.q);
+    __syncthreads();
+    for (int i = k_begin; i < end; ++i) dkv_block<DT, DP, 1, 1, true>(p, i - q_blocks, sh.k);
 }
 
 // sums of the ranges of a split launch, in their order: part [split][rows][D] -> rows of a [B, T, H, D] tensor.  Packed as the kept queries are, or plain
@@ -320,6 +426,18 @@ __global__ __launch_bounds__(256) void attn_lse_sum_kernel(Args p, int keys) {
         const Ten& w = i ? p.w1 : p.w0;
         st4<DT>(const_cast<char*>(w.p) + b * w.b + h * w.h + t * w.t, d, v);
     }
+}
+
+// waves of the launches that form dQ and dK
+long long q_waves(const QPlan& pq) { return pq.blocks * pq.splits * 4; }
+long long k_waves(const Cover& pk, int DP) { return pk.blocks * pk.splits * 4 / (two_roles(DP) ? 2 : 1); }
+
+// what lies in the workspace before the partial results: 16-byte multiples.  (The key launch's plan goes by `causal`; the workspace holds either.)
+long long stats_floats(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int DP, const QPlan& pq) {
+    const long long rows = 2LL * B * Hq * ((Tq + 127LL) / 128 * 128);
+    if (dtype != 1) return rows;
+    const long long k0 = k_waves(k_plan(dtype, B, Tq, Tk, Hq, Hkv, DP, 0), DP), k1 = k_waves(k_plan(dtype, B, Tq, Tk, Hq, Hkv, DP, 1), DP);
+    return rows + q_waves(pq) + (k0 > k1 ? k0 : k1);
 }
 
 template <int DTYPE, int DP>
@@ -348,11 +466,25 @@ void launch_bwd(const Args& a, const Ten& dq, const Ten& dk, const Ten& dv, hipS
     x.splits = pk.splits;
     x.part1 = x.part0 + (long long)pk.splits * a.B * a.Hkv * a.Tk * a.D;
     const dim3 gk((unsigned)(pk.blocks * pk.splits));
+    x.lost_k = a.lost_q + q_waves(pq);
     if (pk.rs == 1) hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, 1>), gk, wg, 0, s, x);
     else hipLaunchKernelGGL((attn_lse_dkv_kernel<DT, DP, FEW>), gk, wg, 0, s, x);
     if (pk.splits > 1) {
         const long long items = (long long)a.B * a.Hkv * a.Tk * (a.D / 4);
         hipLaunchKernelGGL(attn_lse_sum_kernel<DTYPE>, dim3((unsigned)((items + 255) / 256)), wg, 0, s, x, 1);
+    }
+    if constexpr (Tr<DT>::PSHIFT > 0) {
+        constexpr int COLS = 4 * Tr<DT>::TILE;
+        const int qb = a.B * a.Hq * ((a.Tq + COLS - 1) / COLS), kb = a.B * a.Hkv * ((a.Tk + COLS - 1) / COLS);
+        x.w0 = dq;
+        x.w1 = dk;
+        x.splits = 1;
+        x.split_rows = a.split_rows;
+        x.stripes = 1;
+        x.lost_qn = (int)(q_waves(pq) / ((long long)a.B * a.Hkv));
+        x.lost_kn = (int)(k_waves(pk, DP) / ((long long)a.B * a.Hkv));
+        const int per = (qb + kb + 255) / 256;
+        hipLaunchKernelGGL((attn_lse_again_kernel<DT, DP>), dim3((unsigned)((qb + kb + per - 1) / per)), wg, 0, s, x, qb, qb + kb, per);
     }
 }
 template <int DTYPE>
@@ -371,7 +503,7 @@ extern "C" long long dp_attention_lse_bwd_workspace(int dtype, int B, int Tq, in
     const int DP = al::padded_dim(D);
     const al::QPlan pq = al::q_plan(dtype, B, Tq, Tk, Hq, Hkv, DP);
     const al::Cover pk = al::k_plan(dtype, B, Tq, Tk, Hq, Hkv, DP, 1), pk0 = al::k_plan(dtype, B, Tq, Tk, Hq, Hkv, DP, 0);
-    const long long rows = 2LL * B * Hq * ((Tq + 127LL) / 128 * 128);
+    const long long rows = stats_floats(dtype, B, Tq, Tk, Hq, Hkv, DP, pq);
     const long long q = pq.splits > 1 ? (long long)pq.splits * B * Hq * Tq * D : 0;
     const int ks = pk.splits > pk0.splits ? pk.splits : pk0.splits;
     const long long k = ks > 1 ? 2LL * ks * B * Hkv * Tk * D : 0;
@@ -401,7 +533,9 @@ extern "C" int dp_attention_lse_bwd(const void* dout, const void* q, const void*
     DP_REQUIRE(dq != dk && dq != dv && dk != dv, "%s: dq, dk and dv begin at one address", fn);        // (views of one tensor interleave)
     a.lse = const_cast<float*>(lse);
     a.rows = static_cast<float*>(work);
-    a.part0 = a.rows + 2LL * B * Hq * a.Tqp;
+    a.lost_q = reinterpret_cast<int*>(a.rows + 2LL * B * Hq * a.Tqp);
+    const int DP = al::padded_dim(D);
+    a.part0 = a.rows + stats_floats(dtype, B, Tq, Tk, Hq, Hkv, DP, al::q_plan(dtype, B, Tq, Tk, Hq, Hkv, DP));
     hipStream_t s = (hipStream_t)stream;
     if (dtype == 0) launch_bwd<0>(a, tq, tk, tv, s);
     else if (dtype == 1) launch_bwd<1>(a, tq, tk, tv, s);

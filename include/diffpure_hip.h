@@ -410,7 +410,8 @@ int dp_resize_affine_bwd(const float* dy, int B, int C, int Ho, int Wo, int out_
  *   q, out, dout, dq: [B][Tq][Hq][D]     k, v, dk, dv: [B][Tk][Hkv][D]     any strides; channels contiguous.  Hq a multiple of Hkv: query head h
  *     reads key head h / (Hq / Hkv), whose gradient is the sum over the heads that share it.  D a multiple of 8 up to 256.
  *   dtype 0 = fp32 (fp32 matrix products throughout), 1 = fp16, 2 = bf16 (16-bit operands, fp32 scores, sums and gradients in flight; the
- *     probabilities and dS are rounded to the type as operands of their products): one type for all of these tensors; lse is fp32 [B][Hq][Tq].
+ *     probabilities and dS are rounded to the type as operands of their products; in fp16 dS = P (dP - delta) is carried times a power of two, so that neither a
+ *     scaled loss nor small cotangents leave its range: gradients overflow only where they themselves pass 65504): one type for all of these tensors; lse is fp32 [B][Hq][Tq].
  *   strides: HOST array, 3 per tensor (batch, token, head) in elements, multiples of 16 bytes - forward: q, k, v, out (12 values); backward: q, k, v,
  *     out, dout, dq, dk, dv (24 values).  Base pointers 16-byte aligned.  A read tensor may have stride 0 (an expanded one).  So q, k, v and their
  *     gradients may be views of one [B][T][3C] tensor in either head order (dp_attention_fused's layouts).
