@@ -683,11 +683,34 @@ void no_second(const char* name) {
 }
 Tensor or_undefined(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
+// The four operators through the dispatcher: below autograd a call still passes the modes (tracing, fake tensors) that the caller has set
+std::tuple<Tensor, Tensor> call_attention_lse(const Tensor& q, const Tensor& k, const Tensor& v, c10::optional<double> scale, bool causal, const c10::optional<Tensor>& q_lens,
+                                              const c10::optional<Tensor>& kv_lens) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("diffpure_hip::attention_lse", "").typed<decltype(attention_lse)>();
+    return op.call(q, k, v, scale, causal, q_lens, kv_lens);
+}
+std::tuple<Tensor, Tensor, Tensor> call_attention_lse_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse,
+                                                          c10::optional<double> scale, bool causal, const c10::optional<Tensor>& q_lens,
+                                                          const c10::optional<Tensor>& kv_lens) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("diffpure_hip::attention_lse_bwd", "").typed<decltype(attention_lse_bwd)>();
+    return op.call(dout, q, k, v, out, lse, scale, causal, q_lens, kv_lens);
+}
+std::tuple<Tensor, Tensor> call_layer_norm(const Tensor& x, const c10::optional<Tensor>& gamma, const c10::optional<Tensor>& beta, double eps) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("diffpure_hip::layer_norm", "").typed<decltype(layer_norm)>();
+    return op.call(x, gamma, beta, eps);
+}
+std::tuple<Tensor, Tensor, Tensor> call_layer_norm_bwd(const Tensor& dy, const Tensor& x, const c10::optional<Tensor>& gamma, const Tensor& stats,
+                                                       const c10::optional<Tensor>& addend, bool weights) {
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("diffpure_hip::layer_norm_bwd", "").typed<decltype(layer_norm_bwd)>();
+    return op.call(dy, x, gamma, stats, addend, weights);
+}
+c10::optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
+
 struct AttentionLseFn : public torch::autograd::Function<AttentionLseFn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, c10::optional<double> scale, bool causal,
                                  const c10::optional<Tensor>& q_lens, const c10::optional<Tensor>& kv_lens) {
         at::AutoDispatchBelowADInplaceOrView g;
-        auto [out, lse] = attention_lse(q, k, v, scale, causal, q_lens, kv_lens);
+        auto [out, lse] = call_attention_lse(q, k, v, scale, causal, q_lens, kv_lens);
         ctx->save_for_backward({q, k, v, out, lse, or_undefined(q_lens), or_undefined(kv_lens)});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["causal"] = causal;
@@ -699,8 +722,8 @@ struct AttentionLseFn : public torch::autograd::Function<AttentionLseFn> {
         variable_list none(7);
         if (!grads[0].defined()) return none;
         const auto s = ctx->get_saved_variables();
-        auto [dq, dk, dv] = attention_lse_bwd(readable(grads[0]), s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toOptional<double>(),
-                                              ctx->saved_data["causal"].toBool(), s[5], s[6]);
+        auto [dq, dk, dv] = call_attention_lse_bwd(readable(grads[0]), s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toOptional<double>(),
+                                                   ctx->saved_data["causal"].toBool(), if_defined(s[5]), if_defined(s[6]));
         none[0] = dq;
         none[1] = dk;
         none[2] = dv;
@@ -711,7 +734,7 @@ std::tuple<Tensor, Tensor> attention_lse_autograd(const Tensor& q, const Tensor&
                                                   const c10::optional<Tensor>& q_lens, const c10::optional<Tensor>& kv_lens) {
     if (!any_grad({&q, &k, &v})) {
         at::AutoDispatchBelowADInplaceOrView g;
-        return attention_lse(q, k, v, scale, causal, q_lens, kv_lens);
+        return call_attention_lse(q, k, v, scale, causal, q_lens, kv_lens);
     }
     auto r = AttentionLseFn::apply(q, k, v, scale, causal, q_lens, kv_lens);
     return {r[0], r[1]};
@@ -721,7 +744,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& gamma_, const c10::optional<Tensor>& beta_, double eps) {
         at::AutoDispatchBelowADInplaceOrView g;
         const Tensor gamma = or_undefined(gamma_), beta = or_undefined(beta_);
-        auto [y, stats] = layer_norm(x, gamma_, beta_, eps);
+        auto [y, stats] = call_layer_norm(x, gamma_, beta_, eps);
         ctx->save_for_backward({x, gamma, stats});
         const bool wg = gamma.defined() && gamma.requires_grad(), wb = beta.defined() && beta.requires_grad();
         ctx->saved_data["weights"] = wg || wb;
@@ -737,7 +760,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
         const auto s = ctx->get_saved_variables();
         Tensor dy = grads[0];
         if (dy.dim() > 1 || dy.stride(-1) != 1) dy = dy.contiguous();
-        auto [dx, dgamma, dbeta] = layer_norm_bwd(dy, s[0], s[1], s[2], c10::nullopt, ctx->saved_data["weights"].toBool());
+        auto [dx, dgamma, dbeta] = call_layer_norm_bwd(dy, s[0], if_defined(s[1]), s[2], c10::nullopt, ctx->saved_data["weights"].toBool());
         none[0] = dx;
         if (s[1].defined()) none[1] = dgamma;
         if (ctx->saved_data["has_beta"].toBool() && dbeta.defined()) none[2] = dbeta.to((at::ScalarType)ctx->saved_data["beta_type"].toInt());
@@ -748,7 +771,7 @@ std::tuple<Tensor, Tensor> layer_norm_autograd(const Tensor& x, const c10::optio
     const Tensor ga = or_undefined(gamma), be = or_undefined(beta);
     if (!any_grad({&x, &ga, &be})) {
         at::AutoDispatchBelowADInplaceOrView g;
-        return layer_norm(x, gamma, beta, eps);
+        return call_layer_norm(x, gamma, beta, eps);
     }
     auto r = LayerNormFn::apply(x, gamma, beta, eps);
     return {r[0], r[1]};
