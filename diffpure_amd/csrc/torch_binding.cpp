@@ -672,7 +672,10 @@ Tensor readable(const Tensor& g) {
     ok = ok && reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
     return ok ? g : g.clone(at::MemoryFormat::Contiguous);
 }
+// whether a call concerns automatic differentiation; a tensor with a tangent does (there is no forward-mode formula: Function::apply says so)
 bool any_grad(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) return true;
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : ts)
         if (t->defined() && t->requires_grad()) return true;

@@ -109,3 +109,18 @@ def test_without_a_mode_a_cpu_tensor_is_refused():
             fw().attention_lse(*qkv(grad))
         with pytest.raises((RuntimeError, NotImplementedError), match="GPU tensor|CPU"):
             fw().layer_norm(torch.randn(4, 16, requires_grad=grad))
+
+
+@pytest.mark.parametrize("which", range(6))
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_is_refused_not_lost(which, grad_mode):
+    """a dual tensor in any place, without requires_grad: there is no formula for its tangent (nor has the older operators'), and the call says so"""
+    from torch.autograd import forward_ad as fa
+    a = qkv(False) + [torch.randn(2, 5, 16), torch.randn(16), torch.randn(16)]
+    with fa.dual_level(), Answer(), torch.set_grad_enabled(grad_mode):
+        a[which] = fa.make_dual(a[which], torch.ones_like(a[which]))
+        with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward"):
+            if which < 3:
+                fw().attention_lse(*a[:3])
+            else:
+                fw().layer_norm(a[3], a[4], a[5], 1e-6)
