@@ -665,10 +665,12 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy, const Tensor
     return {dx, dgamma, dbeta};
 }
 
-// a cotangent as the kernels read it: channels contiguous, every pitch a multiple of 16 bytes (an expanded one, as sum() leaves it, is laid out)
+// a cotangent [B, T, H, D] as the kernels read it: channels contiguous, every pitch a multiple of 16 bytes, tokens at most 2^24 bytes apart (an expanded one, as sum()
+// leaves it, is laid out)
 Tensor readable(const Tensor& g) {
     bool ok = g.size(-1) <= 1 || g.stride(-1) == 1;
     for (int64_t i = 0; i + 1 < g.dim(); ++i) ok = ok && (g.size(i) <= 1 || g.stride(i) * (int64_t)g.element_size() % 16 == 0);
+    ok = ok && (g.size(1) <= 1 || g.stride(1) * (int64_t)g.element_size() <= 1 << 24);
     ok = ok && reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
     return ok ? g : g.clone(at::MemoryFormat::Contiguous);
 }

@@ -124,3 +124,31 @@ def test_forward_mode_is_refused_not_lost(which, grad_mode):
                 fw().attention_lse(*a[:3])
             else:
                 fw().layer_norm(a[3], a[4], a[5], 1e-6)
+
+
+def test_a_cotangent_is_handed_on_as_the_kernel_takes_it():
+    """whatever its strides (autograd passes a view on as it is): expanded, transposed, beside a 16-byte border, tokens further apart than the kernel takes"""
+    q = torch.randn(1, 3, 2, 8, requires_grad=True)
+    k, v = torch.randn(1, 4, 2, 8), torch.randn(1, 4, 2, 8)
+    wide = torch.zeros(3 * 4500000)                       # 18 MB between two tokens
+    cases = [torch.ones(1).expand(1, 3, 2, 8), torch.randn(1, 3, 8, 2).transpose(2, 3), torch.randn(49)[1:].view(1, 3, 2, 8), torch.randn(1, 3, 2, 9)[..., :8],
+             wide.as_strided((1, 3, 2, 8), (0, 4500000, 8, 1)), torch.randn(1, 2, 3, 8).transpose(1, 2), torch.randn(1, 1, 2, 8).expand(1, 3, 2, 8)]
+    got = []
+
+    class Look(Answer):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if func.name().endswith("attention_lse_bwd"):
+                got.append(args[0])
+            return super().__torch_dispatch__(func, types, args, kwargs)
+
+    for c in cases:
+        with Look():
+            torch.autograd.grad(fw().attention_lse(q, k, v)[0], q, c)
+        g = got.pop()
+        assert torch.equal(g, c)
+        assert g.stride(3) == 1 and g.data_ptr() % 16 == 0 and all(g.stride(i) * 4 % 16 == 0 for i in range(3) if g.shape[i] > 1), g.stride()
+        assert g.stride(1) * 4 <= 1 << 24, g.stride()
+    for c in cases[5:]:                                   # what it takes is not copied
+        with Look():
+            torch.autograd.grad(fw().attention_lse(q, k, v)[0], q, c)
+        assert got.pop().data_ptr() == c.data_ptr()
