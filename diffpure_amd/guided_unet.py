@@ -594,7 +594,7 @@ class GuidedUNet:
         da = self._dconv(dout, n + ".dwproj", r.get("dh2_p", False) == "h1" and "h1", c, 1)
         h16_ok = getattr(self, "_gpool", None) is not None and os.environ.get("DIFFPURE_ATTN_BWD16", "1") != "0"
         qkv = t["qkv"]
-        if ops.attention_recompute_wanted():
+        if ops.attention_recompute_wanted(c // r["heads"]):
             dqkv = ops.attention_recompute_bwd(qkv.view(b, hh * ww, 3 * c), da.view(b, hh * ww, c), r["heads"], t["layout"])
             dxn = self._dconv(dqkv.view(b, hh, ww, 3 * c), n + ".dwqkv", r["dh2"], c, 1)
             return ops.group_norm_bwd(t["x"], self.GN_GROUPS, P[n + ".g"], P[n + ".b"], t["st"], dxn, addend=dout)[0]

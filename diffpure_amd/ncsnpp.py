@@ -547,7 +547,7 @@ class NCSNpp:
         da = self._dconv(dout, n + ".dw3", r.get("dh2_3", False) == "h1" and "h1", c, 1, scale=INV_SQRT2)
         h16_ok = getattr(self, "_gpool", None) is not None and os.environ.get("DIFFPURE_ATTN_BWD16", "1") != "0"
         qkv = t["qkv"]
-        if ops.attention_recompute_wanted():
+        if ops.attention_recompute_wanted(c):
             dqkv = ops.attention_recompute_bwd(qkv.view(b, hh * ww, 3 * c), da.view(b, hh * ww, c), 1, "split")
             dhn = self._dconv(dqkv.view(b, hh, ww, 3 * c), n + ".dwqkv", r["dh2"], c, 1)
             return ops.group_norm_bwd(t["x"], self._groups(c), P[n + ".g"], P[n + ".b"], t["st"], dhn, addend=dout, addend_scale=INV_SQRT2)[0]

@@ -1140,10 +1140,11 @@ def attention_lse_bwd(dout, q, k, v, out, lse, scale=None, causal=False, q_lens=
     return dq, dk, dv
 
 
-def attention_recompute_wanted():
+def attention_recompute_wanted(d):
     """DIFFPURE_ATTN_RECOMPUTE=1: the engines' attention backward (adjoint workloads) runs on attention_lse / attention_lse_bwd: no [B * heads, T, T]
-    tensors (two of 2.1 GB per 32 x 32 layer at B = 64).  Off by default: the low-order bits differ from the product-by-product form."""
-    return os.environ.get("DIFFPURE_ATTN_RECOMPUTE", "0") == "1"
+    tensors (two of 2.1 GB per 32 x 32 layer at B = 64).  Off by default: the low-order bits differ from the product-by-product form - which layers whose
+    head dimension d attention_lse does not take (no multiple of 8, or above 256) keep in any case."""
+    return d % 8 == 0 and d <= 256 and os.environ.get("DIFFPURE_ATTN_RECOMPUTE", "0") == "1"
 
 
 def attention_recompute_bwd(qkv, dout, n_heads, layout):
