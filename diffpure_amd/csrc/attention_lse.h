@@ -284,6 +284,11 @@ template <int DT> __device__ __forceinline__ void st4(char* rowp, int d, f32x4 v
     for (int j = 0; j < 4; ++j) e[j] = (typename Tr<DT>::E)v[j];
     *reinterpret_cast<typename Tr<DT>::E4*>(rowp + (long long)d * Tr<DT>::ES) = e;
 }
+// ... or in fp32 whatever the type is
+template <int DT> __device__ __forceinline__ void st4(char* rowp, int d, f32x4 v, int wide) {
+    if (wide) *reinterpret_cast<f32x4*>(rowp + (long long)d * 4) = v;
+    else st4<DT>(rowp, d, v);
+}
 // The waves that took different rows for the same columns (RS of them, rank rw) join their accumulators: every wave leaves its units in LDS and sums a
 // share of them, in the order of the ranks.  sink(unit, sum) gets each unit once.  smem: Units::N KB per wave; a barrier must lie before the call.
 template <int DT, int ND, int RS, typename Sink>
@@ -356,6 +361,7 @@ struct Args {
     float* part_lse;              // forward: [split][kept row]
     const int *q_lens, *kv_lens;
     int B, Tq, Tk, Hq, Hkv, D, Tqp;
+    int wide;                     // backward: the gradients are fp32 whatever the operands are
     int packed;                   // 1: the queries of all heads of a group are the columns of one block (heads share their keys)
     int splits, split_rows;       // the streamed rows are cut into `splits` ranges of split_rows
     float scale;
@@ -482,6 +488,7 @@ inline Cover k_plan(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int DP, i
 
 // argument checks shared by the two entry points (attention_lse.hip): message and non-zero / false on a refusal
 bool dp_attn_lse_tensor(const char* fn, const char* name, const void* ptr, const long long* st, int es, int B, int Tn, int H, bool written, al::Ten* t);
-bool dp_attn_lse_apart(const char* fn, const char* name, const al::Ten& w, int wt, int wh, const char* other, const al::Ten& r, int rt, int rh, int B, long long row);
+bool dp_attn_lse_apart(const char* fn, const char* name, const al::Ten& w, int wt, int wh, const char* other, const al::Ten& r, int rt, int rh, int B, long long wrow,
+                        long long rrow);
 int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq,
                        int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, al::Args* a);

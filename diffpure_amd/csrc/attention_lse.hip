@@ -244,8 +244,9 @@ bool dp_attn_lse_tensor(const char* fn, const char* name, const void* ptr, const
 }
 
 // a written tensor against a read one: their bytes from first to last must lie apart, or their tokens must be different columns of rows at one pitch
-bool dp_attn_lse_apart(const char* fn, const char* name, const al::Ten& w, int wt, int wh, const char* other, const al::Ten& r, int rt, int rh, int B, long long row) {
-    const long long ww = (wh - 1LL) * w.h + row, rw = (rh - 1LL) * r.h + row;                  // a token's bytes, its heads apart or side by side
+bool dp_attn_lse_apart(const char* fn, const char* name, const al::Ten& w, int wt, int wh, const char* other, const al::Ten& r, int rt, int rh, int B, long long wrow,
+                        long long rrow) {
+    const long long ww = (wh - 1LL) * w.h + wrow, rw = (rh - 1LL) * r.h + rrow;                  // a token's bytes, its heads apart or side by side
     const long long wend = (B - 1LL) * w.b + (wt - 1LL) * w.t + ww, rend = (B - 1LL) * r.b + (rt - 1LL) * r.t + rw, at = (intptr_t)r.p - (intptr_t)w.p;
     if (at >= wend || -at >= rend) return true;
     const bool one = wt == 1 && rt == 1;                                                       // single tokens: a row of each sample
@@ -302,8 +303,8 @@ extern "C" int dp_attention_lse(const void* q, const void* k, const void* v, con
     const long long need = dp_attention_lse_workspace(dtype, B, Tq, Tk, Hq, Hkv, D);
     DP_REQUIRE(need == 0 || (work && dp_aligned16(work) && work_bytes >= need), "%s: workspace of %lld bytes needed (got %lld)", fn, need, work_bytes);
     const long long row = (long long)D * (dtype == 0 ? 4 : 2);
-    if (!dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "q", a.q, Tq, Hq, B, row) || !dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "k", a.k, Tk, Hkv, B, row) ||
-        !dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "v", a.v, Tk, Hkv, B, row))
+    if (!dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "q", a.q, Tq, Hq, B, row, row) || !dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "k", a.k, Tk, Hkv, B, row, row) ||
+        !dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "v", a.v, Tk, Hkv, B, row, row))
         return 1;
     a.lse = lse;
     a.part0 = static_cast<float*>(work);

@@ -27,8 +27,10 @@ template <int DT, int DP, int RS> struct Dq {
     using St = Stream<DP * Tr<DT>::ES, Tr<DT>::ES, RS * Tr<DT>::ROWS, 4>;
     struct Shared { char stage[2 * St::STAGE]; };
 };
-// an element of a written tensor that is infinite or NaN
-__device__ __forceinline__ bool not_finite16(const char* x) { return (*reinterpret_cast<const unsigned short*>(x) & 0x7c00) == 0x7c00; }
+// an fp16 (or, wide, fp32) element of a written tensor that is infinite or NaN
+__device__ __forceinline__ bool not_finite(const char* x, int wide) {
+    return wide ? (*reinterpret_cast<const unsigned*>(x) & 0x7f800000) == 0x7f800000 : (*reinterpret_cast<const unsigned short*>(x) & 0x7c00) == 0x7c00;
+}
 
 // dQ.  Workgroups, stages and RS as in the forward kernel.  AGAIN: the queries among the workgroup's whose dq (all of a query's channels, or none) is not finite.
 template <int DT, int DP, int RS, bool AGAIN>
@@ -56,7 +58,7 @@ __device__ __forceinline__ void dq_block(const Args& p, int bid0, typename Dq<DT
     kept.col(p, col < kept.cols ? col : kept.cols - 1, head, tok);
     bool lost = false;
     if constexpr (AGAIN) {
-        lost = not_finite16(p.w0.p + b * p.w0.b + head * p.w0.h + tok * p.w0.t);
+        lost = not_finite(p.w0.p + b * p.w0.b + head * p.w0.h + tok * p.w0.t, p.wide);
         if (!__syncthreads_or(lost)) return;
     }
     const int krow = tok < n ? tok : (n > 0 ? n - 1 : 0);
@@ -168,9 +170,9 @@ __device__ __forceinline__ void dq_block(const Args& p, int bid0, typename Dq<DT
     if constexpr (AGAIN) {
         join_units<DT, ND, 1>(dq, mul, smem, wave, 0, lane, [&](int u, f32x4 v) {
             const int d = Units<DT, ND>::d(u, g);
-            if (out && lost && d < p.D) st4<DT>(row, d, v);
+            if (out && lost && d < p.D) st4<DT>(row, d, v, p.wide);
         });
-    } else if (RS == 1 && p.splits == 1) {
+    } else if (RS == 1 && p.splits == 1 && !p.wide) {
         __syncthreads();
         const int first = c0 + wave * T::TILE;
         store_cols<DT, ND, RB>(dq, mul, smem + wave * T::TILE * RB, lane, row_slots, [&](int i) -> char* {
@@ -182,7 +184,7 @@ __device__ __forceinline__ void dq_block(const Args& p, int bid0, typename Dq<DT
         const int d = Units<DT, ND>::d(u, g);
         if (!out || d >= p.D) return;
         if (p.splits > 1) *reinterpret_cast<f32x4*>(p.part0 + kr * p.D + d) = v;
-        else st4<DT>(row, d, v);
+        else st4<DT>(row, d, v, p.wide);
     });
 }
 
@@ -225,7 +227,7 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
 
     bool lost = false;
     if constexpr (AGAIN) {
-        lost = not_finite16(p.w1.p + b * p.w1.b + hk * p.w1.h + (col < p.Tk ? col : p.Tk - 1) * p.w1.t);
+        lost = not_finite(p.w1.p + b * p.w1.b + hk * p.w1.h + (col < p.Tk ? col : p.Tk - 1) * p.w1.t, p.wide);
         if (!__syncthreads_or(lost)) return;
     }
     typename T::Frag kf[KS], vf[DK ? KS : 1];
@@ -334,7 +336,7 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
             const bool found = lost && fabsf(dk[0][0]) < INFINITY;
             join_units<DT, ND, 1>(dk, col < m ? ldexpf(p.scale, low - T::PSHIFT) : 0.f, smem, wave, 0, lane, [&](int u, f32x4 v) {
                 const int d = Units<DT, ND>::d(u, g);
-                if (found && col < p.Tk && d < p.D) st4<DT>(row, d, v);
+                if (found && col < p.Tk && d < p.D) st4<DT>(row, d, v, p.wide);
             });
             lost = lost && !found;
         } while (__syncthreads_or(lost && low < 36));
@@ -354,7 +356,7 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
     const long long kr = ((long long)split * p.B * p.Hkv + z) * p.Tk + col;
     auto put = [&](const typename T::Acc(&acc)[ND], float mul, const Ten& w, float* part) {
         __syncthreads();
-        if (RS == 1 && p.splits == 1) {
+        if (RS == 1 && p.splits == 1 && !p.wide) {
             const int first = c0 + wave * T::TILE;
             store_cols<DT, ND, RB>(acc, mul, smem + wave * T::TILE * RB, lane, row_slots, [&](int i) -> char* {
                 return first + i < p.Tk ? const_cast<char*>(w.p) + b * w.b + hk * w.h + (first + i) * w.t : nullptr;
@@ -363,7 +365,7 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
             const int d = Units<DT, ND>::d(u, g);
             if (!out || d >= p.D) return;
             if (p.splits > 1) *reinterpret_cast<f32x4*>(part + kr * p.D + d) = v;
-            else st4<DT>(const_cast<char*>(w.p) + b * w.b + hk * w.h + col * w.t, d, v);
+            else st4<DT>(const_cast<char*>(w.p) + b * w.b + hk * w.h + col * w.t, d, v, p.wide);
         });
     };
     if constexpr (DK) put(dk, p.scale * pm, p.w0, p.part0);
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(256) void attn_lse_sum_kernel(Args p, int keys) {
         f32x4 v = *reinterpret_cast<const f32x4*>(part);
         for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const f32x4*>(part + s * rows * p.D);
         const Ten& w = i ? p.w1 : p.w0;
-        st4<DT>(const_cast<char*>(w.p) + b * w.b + h * w.h + t * w.t, d, v);
+        st4<DT>(const_cast<char*>(w.p) + b * w.b + h * w.h + t * w.t, d, v, p.wide);
     }
 }
 
@@ -510,18 +512,18 @@ extern "C" long long dp_attention_lse_bwd_workspace(int dtype, int B, int Tq, in
     return (rows + (q > k ? q : k)) * 4;                // the partial sums of dQ are read before those of dK and dV are written
 }
 
-extern "C" int dp_attention_lse_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides,
-                                    int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal,
-                                    void* dq, void* dk, void* dv, void* work, long long work_bytes, void* stream) {
-    const char* fn = "dp_attention_lse_bwd";
+namespace {
+int attn_lse_bwd(const char* fn, bool wide, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides,
+                 int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, void* dq, void* dk, void* dv,
+                 void* work, long long work_bytes, void* stream) {
     al::Args a{};
     if (int rc = dp_attn_lse_common(fn, q, k, v, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, &a)) return rc;
-    const int es = dtype == 0 ? 4 : 2;
+    const int es = dtype == 0 ? 4 : 2, ges = wide ? 4 : es;
     al::Ten tq, tk, tv;
     DP_REQUIRE(lse, "%s: lse missing", fn);
     if (!dp_attn_lse_tensor(fn, "out", out, strides + 9, es, B, Tq, Hq, false, &a.o) || !dp_attn_lse_tensor(fn, "dout", dout, strides + 12, es, B, Tq, Hq, false, &a.dout) ||
-        !dp_attn_lse_tensor(fn, "dq", dq, strides + 15, es, B, Tq, Hq, true, &tq) || !dp_attn_lse_tensor(fn, "dk", dk, strides + 18, es, B, Tk, Hkv, true, &tk) ||
-        !dp_attn_lse_tensor(fn, "dv", dv, strides + 21, es, B, Tk, Hkv, true, &tv))
+        !dp_attn_lse_tensor(fn, "dq", dq, strides + 15, ges, B, Tq, Hq, true, &tq) || !dp_attn_lse_tensor(fn, "dk", dk, strides + 18, ges, B, Tk, Hkv, true, &tk) ||
+        !dp_attn_lse_tensor(fn, "dv", dv, strides + 21, ges, B, Tk, Hkv, true, &tv))
         return 1;
     const long long need = dp_attention_lse_bwd_workspace(dtype, B, Tq, Tk, Hq, Hkv, D);
     DP_REQUIRE(work && dp_aligned16(work) && work_bytes >= need, "%s: workspace of %lld bytes needed (got %lld)", fn, need, work_bytes);
@@ -529,8 +531,9 @@ extern "C" int dp_attention_lse_bwd(const void* dout, const void* q, const void*
         rd[5] = {{"q", a.q, Tq, Hq}, {"k", a.k, Tk, Hkv}, {"v", a.v, Tk, Hkv}, {"out", a.o, Tq, Hq}, {"dout", a.dout, Tq, Hq}};
     for (const auto& w : wr)
         for (const auto& r : rd)
-            if (!dp_attn_lse_apart(fn, w.name, w.t, w.tokens, w.heads, r.name, r.t, r.tokens, r.heads, B, (long long)D * es)) return 1;
+            if (!dp_attn_lse_apart(fn, w.name, w.t, w.tokens, w.heads, r.name, r.t, r.tokens, r.heads, B, (long long)D * ges, (long long)D * es)) return 1;
     DP_REQUIRE(dq != dk && dq != dv && dk != dv, "%s: dq, dk and dv begin at one address", fn);        // (views of one tensor interleave)
+    a.wide = wide && dtype != 0;
     a.lse = const_cast<float*>(lse);
     a.rows = static_cast<float*>(work);
     a.lost_q = reinterpret_cast<int*>(a.rows + 2LL * B * Hq * a.Tqp);
@@ -542,4 +545,18 @@ extern "C" int dp_attention_lse_bwd(const void* dout, const void* q, const void*
     else launch_bwd<2>(a, tq, tk, tv, s);
     DP_LAUNCH_CHECK("attn_lse_bwd");
     return 0;
+}
+}  // namespace
+
+extern "C" int dp_attention_lse_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides,
+                                    int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal,
+                                    void* dq, void* dk, void* dv, void* work, long long work_bytes, void* stream) {
+    return attn_lse_bwd("dp_attention_lse_bwd", false, dout, q, k, v, out, lse, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, dq, dk, dv, work,
+                        work_bytes, stream);
+}
+extern "C" int dp_attention_lse_bwd_f32(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides,
+                                        int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal,
+                                        float* dq, float* dk, float* dv, void* work, long long work_bytes, void* stream) {
+    return attn_lse_bwd("dp_attention_lse_bwd_f32", true, dout, q, k, v, out, lse, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, dq, dk, dv, work,
+                        work_bytes, stream);
 }
