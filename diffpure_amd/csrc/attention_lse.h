@@ -12,6 +12,7 @@
 // fp32 runs on the fp32 matrix instruction (16 x 16 x 4): full fp32 products, no splitting, no range limits.
 #pragma once
 #include "dp_common.h"
+#include "dp_region.h"
 #include "dp_tune.h"
 
 namespace al {
@@ -488,7 +489,6 @@ inline Cover k_plan(int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int DP, i
 
 // argument checks shared by the two entry points (attention_lse.hip): message and non-zero / false on a refusal
 bool dp_attn_lse_tensor(const char* fn, const char* name, const void* ptr, const long long* st, int es, int B, int Tn, int H, bool written, al::Ten* t);
-bool dp_attn_lse_apart(const char* fn, const char* name, const al::Ten& w, int wt, int wh, const char* other, const al::Ten& r, int rt, int rh, int B, long long wrow,
-                        long long rrow);
+dp::Region dp_attn_lse_region(const char* name, const al::Ten& t, int B, int Tn, int H, long long row);
 int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq,
                        int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, al::Args* a);

@@ -243,20 +243,8 @@ bool dp_attn_lse_tensor(const char* fn, const char* name, const void* ptr, const
     return true;
 }
 
-// a written tensor against a read one: their bytes from first to last must lie apart, or their tokens must be different columns of rows at one pitch
-bool dp_attn_lse_apart(const char* fn, const char* name, const al::Ten& w, int wt, int wh, const char* other, const al::Ten& r, int rt, int rh, int B, long long wrow,
-                        long long rrow) {
-    const long long ww = (wh - 1LL) * w.h + wrow, rw = (rh - 1LL) * r.h + rrow;                  // a token's bytes, its heads apart or side by side
-    const long long wend = (B - 1LL) * w.b + (wt - 1LL) * w.t + ww, rend = (B - 1LL) * r.b + (rt - 1LL) * r.t + rw, at = (intptr_t)r.p - (intptr_t)w.p;
-    if (at >= wend || -at >= rend) return true;
-    const bool one = wt == 1 && rt == 1;                                                       // single tokens: a row of each sample
-    const long long pitch = one ? w.b : w.t;
-    if (pitch > 0 && (one ? r.b : r.t) == pitch && (one || (w.b % pitch == 0 && r.b % pitch == 0))) {
-        const long long col = (at % pitch + pitch) % pitch;                                    // where r's token begins in w's row
-        if (col >= ww && col + rw <= pitch) return true;
-    }
-    dp_set_error("%s: %s overlaps %s", fn, name, other);
-    return false;
+dp::Region dp_attn_lse_region(const char* name, const al::Ten& t, int B, int Tn, int H, long long row) {
+    return dp::Region{name, (intptr_t)t.p, {B, Tn, H}, {t.b, t.t, t.h}, row};
 }
 
 int dp_attn_lse_common(const char* fn, const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq,
@@ -303,9 +291,10 @@ extern "C" int dp_attention_lse(const void* q, const void* k, const void* v, con
     const long long need = dp_attention_lse_workspace(dtype, B, Tq, Tk, Hq, Hkv, D);
     DP_REQUIRE(need == 0 || (work && dp_aligned16(work) && work_bytes >= need), "%s: workspace of %lld bytes needed (got %lld)", fn, need, work_bytes);
     const long long row = (long long)D * (dtype == 0 ? 4 : 2);
-    if (!dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "q", a.q, Tq, Hq, B, row, row) || !dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "k", a.k, Tk, Hkv, B, row, row) ||
-        !dp_attn_lse_apart(fn, "out", a.w0, Tq, Hq, "v", a.v, Tk, Hkv, B, row, row))
-        return 1;
+    const dp::Region written[] = {dp_attn_lse_region("out", a.w0, B, Tq, Hq, row), dp::flat("lse", lse, 4LL * B * Hq * Tq), dp::flat("work", work, need)},
+                     read[] = {dp_attn_lse_region("q", a.q, B, Tq, Hq, row), dp_attn_lse_region("k", a.k, B, Tk, Hkv, row), dp_attn_lse_region("v", a.v, B, Tk, Hkv, row),
+                               dp::flat("q_lens", q_lens, 4LL * B), dp::flat("kv_lens", kv_lens, 4LL * B)};
+    if (dp::check_apart(fn, written, 3, read, 5)) return 1;
     a.lse = lse;
     a.part0 = static_cast<float*>(work);
     a.part_lse = need ? a.part0 + need / 4 / (D + 1) * D : nullptr;

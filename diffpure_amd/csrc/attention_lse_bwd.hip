@@ -527,12 +527,13 @@ int attn_lse_bwd(const char* fn, bool wide, const void* dout, const void* q, con
         return 1;
     const long long need = dp_attention_lse_bwd_workspace(dtype, B, Tq, Tk, Hq, Hkv, D);
     DP_REQUIRE(work && dp_aligned16(work) && work_bytes >= need, "%s: workspace of %lld bytes needed (got %lld)", fn, need, work_bytes);
-    const struct { const char* name; al::Ten t; int tokens, heads; } wr[3] = {{"dq", tq, Tq, Hq}, {"dk", tk, Tk, Hkv}, {"dv", tv, Tk, Hkv}},
-        rd[5] = {{"q", a.q, Tq, Hq}, {"k", a.k, Tk, Hkv}, {"v", a.v, Tk, Hkv}, {"out", a.o, Tq, Hq}, {"dout", a.dout, Tq, Hq}};
-    for (const auto& w : wr)
-        for (const auto& r : rd)
-            if (!dp_attn_lse_apart(fn, w.name, w.t, w.tokens, w.heads, r.name, r.t, r.tokens, r.heads, B, (long long)D * ges, (long long)D * es)) return 1;
-    DP_REQUIRE(dq != dk && dq != dv && dk != dv, "%s: dq, dk and dv begin at one address", fn);        // (views of one tensor interleave)
+    const long long row = (long long)D * es, grow = (long long)D * ges;
+    const dp::Region written[] = {dp_attn_lse_region("dq", tq, B, Tq, Hq, grow), dp_attn_lse_region("dk", tk, B, Tk, Hkv, grow), dp_attn_lse_region("dv", tv, B, Tk, Hkv, grow),
+                                  dp::flat("work", work, need)},
+                     read[] = {dp_attn_lse_region("q", a.q, B, Tq, Hq, row), dp_attn_lse_region("k", a.k, B, Tk, Hkv, row), dp_attn_lse_region("v", a.v, B, Tk, Hkv, row),
+                               dp_attn_lse_region("out", a.o, B, Tq, Hq, row), dp_attn_lse_region("dout", a.dout, B, Tq, Hq, row), dp::flat("lse", lse, 4LL * B * Hq * Tq),
+                               dp::flat("q_lens", q_lens, 4LL * B), dp::flat("kv_lens", kv_lens, 4LL * B)};
+    if (dp::check_apart(fn, written, 4, read, 8)) return 1;
     a.wide = wide && dtype != 0;
     a.lse = const_cast<float*>(lse);
     a.rows = static_cast<float*>(work);

@@ -423,8 +423,9 @@ int dp_resize_affine_bwd(const float* dy, int B, int C, int Ho, int Wo, int out_
  *     and dk, dv of the keys it sees, are NaN.
  *   scale: finite, not 0.
  *   work: dp_attention_lse_workspace / dp_attention_lse_bwd_workspace bytes, 16-byte aligned, free again when the call's work on `stream` is done (the
- *     forward pass needs none - 0 - where the queries fill the chip).  The outputs may not overlap any input (refused; columns of
- *     rows at one pitch are apart), nor two gradients begin at one address.  Tokens of a tensor lie at most 2^24
+ *     forward pass needs none - 0 - where the queries fill the chip).  Whatever a call writes (gradients, out, lse, work) lies
+ *     apart from everything that it reads and else writes, and a written tensor's rows from one another: refused where they share bytes (views of one tensor
+ *     that interleave do not). Tokens of a tensor lie at most 2^24
  *     bytes apart.  Results do not depend on the order in which workgroups run (no atomics).
  * The reference has no counterpart that keeps the statistics (QKVAttentionLegacy.forward, guided_diffusion/unet.py:345-362, materialises the weights and
  * autograd keeps or checkpoints them). */
