@@ -13,6 +13,7 @@
 // 29.3 us = 5.3 TB/s; backward with weight gradients and addend 60.4 us = 5.1 TB/s; backward 5 003 x 1001 fp32 16.3 us = 3.7 TB/s (two launches);
 // forward 64 x 768 6 us, the time of a launch.  The variant of plan() goes by the row's width only.
 #include "dp_common.h"
+#include "dp_region.h"
 
 namespace {
 
@@ -349,6 +350,12 @@ int check(const char* fn, int x_dtype, int w_dtype, long long rows, int C) {
     return 0;
 }
 
+constexpr long long MAX_PITCH = 1LL << 40;
+
+dp::Region row_region(const char* name, const void* p, long long rows, int C, long long pitch, int es) {
+    return dp::Region{name, (intptr_t)p, {rows, 1, 1}, {pitch * es, 0, 0}, p ? (long long)C * es : 0};
+}
+
 }  // namespace
 
 extern "C" int dp_layer_norm(const void* x, int x_dtype, long long rows, int C, long long x_stride, const void* gamma, const void* beta, int w_dtype, float eps, void* y,
@@ -357,7 +364,11 @@ extern "C" int dp_layer_norm(const void* x, int x_dtype, long long rows, int C, 
     if (int rc = check(fn, x_dtype, w_dtype, rows, C)) return rc;
     DP_REQUIRE(x && y, "%s: tensor missing", fn);
     DP_REQUIRE(eps >= 0.f && eps - eps == 0.f, "%s: eps must be finite and not negative", fn);
-    DP_REQUIRE(x_stride >= 0 && (y_stride >= C || rows == 1), "%s: row pitch (x %lld, y %lld; y's rows must not overlap)", fn, x_stride, y_stride);
+    DP_REQUIRE(x_stride >= 0 && x_stride <= MAX_PITCH && y_stride <= MAX_PITCH && (y_stride >= C || rows == 1), "%s: row pitch (x %lld, y %lld; y's rows must not overlap)", fn, x_stride, y_stride);
+    const int es = x_dtype == 0 ? 4 : 2, wes = w_dtype == 0 ? 4 : 2;
+    const dp::Region written[] = {row_region("y", y, rows, C, y_stride, es), dp::flat("stats", stats, rows * 8)},
+                     read[] = {row_region("x", x, rows, C, x_stride, es), dp::flat("gamma", gamma, (long long)C * wes), dp::flat("beta", beta, (long long)C * wes)};
+    if (dp::check_apart(fn, written, 2, read, 3)) return 1;
     const FwdCall c{x, rows, C, x_stride, gamma, beta, eps, y, y_stride, stats, (hipStream_t)stream};
     dispatch(c, x_dtype, w_dtype, plan(C, x_dtype == 0 ? 4 : 8));
     DP_LAUNCH_CHECK("layer_norm");
@@ -375,10 +386,17 @@ extern "C" int dp_layer_norm_bwd(const void* dy, long long dy_stride, const void
     const char* fn = "dp_layer_norm_bwd";
     if (int rc = check(fn, x_dtype, w_dtype, rows, C)) return rc;
     DP_REQUIRE(dy && x && stats && dx, "%s: tensor missing", fn);
-    DP_REQUIRE(dy_stride >= 0 && x_stride >= 0 && addend_stride >= 0 && (dx_stride >= C || rows == 1), "%s: row pitch (dx's rows must not overlap)", fn);
+    DP_REQUIRE(dy_stride >= 0 && x_stride >= 0 && addend_stride >= 0 && dy_stride <= MAX_PITCH && x_stride <= MAX_PITCH && addend_stride <= MAX_PITCH && dx_stride <= MAX_PITCH &&
+                   (dx_stride >= C || rows == 1), "%s: row pitch (dx's rows must not overlap)", fn);
     const bool weights = dgamma || dbeta;
     DP_REQUIRE(!weights || (work && (reinterpret_cast<uintptr_t>(work) & 3) == 0 && work_bytes >= dp_layer_norm_bwd_workspace(rows, C, x_dtype)),
                "%s: workspace of %lld bytes needed for the weight gradients (got %lld)", fn, dp_layer_norm_bwd_workspace(rows, C, x_dtype), work_bytes);
+    const int es = x_dtype == 0 ? 4 : 2, wes = w_dtype == 0 ? 4 : 2;
+    const dp::Region written[] = {row_region("dx", dx, rows, C, dx_stride, es), dp::flat("dgamma", dgamma, (long long)C * wes), dp::flat("dbeta", dbeta, (long long)C * wes),
+                                  dp::flat("work", weights ? work : nullptr, dp_layer_norm_bwd_workspace(rows, C, x_dtype))},
+                     read[] = {row_region("dy", dy, rows, C, dy_stride, es), row_region("x", x, rows, C, x_stride, es), dp::flat("gamma", gamma, (long long)C * wes),
+                               dp::flat("stats", stats, rows * 8), row_region("addend", addend, rows, C, addend_stride, es)};
+    if (dp::check_apart(fn, written, 4, read, 5)) return 1;
     hipStream_t s = (hipStream_t)stream;
     const Plan p = plan(C, x_dtype == 0 ? 4 : 8);
     const BwdCall c{dy, dy_stride, x, x_stride, rows, C, gamma, stats, addend, addend_stride, dx, dx_stride, weights ? (float*)work : nullptr, s};

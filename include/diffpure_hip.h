@@ -423,10 +423,9 @@ int dp_resize_affine_bwd(const float* dy, int B, int C, int Ho, int Wo, int out_
  *     and dk, dv of the keys it sees, are NaN.
  *   scale: finite, not 0.
  *   work: dp_attention_lse_workspace / dp_attention_lse_bwd_workspace bytes, 16-byte aligned, free again when the call's work on `stream` is done (the
- *     forward pass needs none - 0 - where the queries fill the chip).  Whatever a call writes (gradients, out, lse, work) lies
- *     apart from everything that it reads and else writes, and a written tensor's rows from one another: refused where they share bytes (views of one tensor
- *     that interleave do not). Tokens of a tensor lie at most 2^24
- *     bytes apart.  Results do not depend on the order in which workgroups run (no atomics).
+ *     forward pass needs none - 0 - where the queries fill the chip).  Whatever a call writes (gradients, out, lse, work)
+ *     lies apart from everything that it reads and else writes, and a written tensor's rows from one another: refused where they share bytes (views of
+ *     one tensor that interleave share none).  Tokens of a tensor lie at most 2^24 bytes apart.  Results do not depend on the order in which workgroups run (no atomics).
  * The reference has no counterpart that keeps the statistics (QKVAttentionLegacy.forward, guided_diffusion/unet.py:345-362, materialises the weights and
  * autograd keeps or checkpoints them). */
 int dp_attention_lse(const void* q, const void* k, const void* v, const long long* strides, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D,
@@ -448,6 +447,7 @@ int dp_attention_lse_bwd_f32(const void* dout, const void* q, const void* k, con
  *     elements (a read tensor may have pitch 0); any element alignment.  gamma, beta (each may be NULL: 1 and 0), dgamma, dbeta (each may be NULL:
  *     not formed): w_dtype 0 = fp32 or x_dtype.  Sums are fp32; the order of the sums is fixed by (rows, C, type).
  *   work: dp_layer_norm_bwd_workspace(rows, C, x_dtype) bytes where dgamma or dbeta is formed, 4-byte aligned.
+ *   Nothing is done in place: what a call writes (y, stats; dx, dgamma, dbeta, work) shares no byte with anything that it reads or else writes (refused).
  * No reference counterpart in the purifier (its norms are GroupNorms); transformer classifiers behind it (utils.py:143-253's zoo) are built on it. */
 int dp_layer_norm(const void* x, int x_dtype, long long rows, int C, long long x_stride, const void* gamma, const void* beta, int w_dtype, float eps, void* y,
                   long long y_stride, float* stats, void* stream);

@@ -162,3 +162,56 @@ def test_usual_views_pass():
     assert lib().dp_attention_lse_bwd(AT["dout"], AT["q"], AT["k"], AT["v"], AT["out"], AT["lse"], C.addressof(st), 1, 1, 1, 1, H, H, D, None, None, 0.25, 0, AT["dq"],
                                       AT["dq"] + 2 * D, AT["dq"], AT["work"], MB, None) != 0
     assert error().endswith("dq and dv begin at one address"), error()
+
+
+ROWS, WIDTH, PITCH = 6, 32, 40
+LN = {n: (i + 64) * MB for i, n in enumerate(("x", "gamma", "beta", "y", "stats", "dy", "addend", "dx", "dgamma", "dbeta", "work"))}
+SIZE = {n: ((ROWS - 1) * PITCH + WIDTH) * 2 for n in ("x", "y", "dy", "addend", "dx")} | {n: WIDTH * 4 for n in ("gamma", "beta", "dgamma", "dbeta")} | {"stats": ROWS * 8, "work": 8}
+
+
+def ln(**at):
+    a = LN | at
+    assert lib().dp_layer_norm(a["x"], 1, ROWS, WIDTH, PITCH, a["gamma"], a["beta"], 0, 1e-6, a["y"], PITCH, a["stats"], None) != 0
+    return error()
+
+
+def ln_bwd(**at):
+    a = LN | at
+    need = lib().dp_layer_norm_bwd_workspace(ROWS, WIDTH, 1)
+    assert lib().dp_layer_norm_bwd(a["dy"], PITCH, a["x"], PITCH, 1, ROWS, WIDTH, a["gamma"], 0, a["stats"], a["addend"], PITCH, a["dx"], PITCH, a["dgamma"], a["dbeta"], a["work"],
+                                   need, None) != 0
+    return error()
+
+
+@pytest.mark.parametrize("call,written,other", [(ln, w, o) for w in ("y", "stats") for o in ("x", "gamma", "beta")] +
+                         [(ln_bwd, w, o) for w in ("dx", "dgamma", "dbeta", "work") for o in ("dy", "x", "gamma", "stats", "addend")])
+def test_layer_norm_results_on_an_input(call, written, other):
+    """the whole, its last bytes, and its first (a row's part counts, the gap behind it does not: see below)"""
+    for off in (0, SIZE[other] - 4, -(SIZE[written] - 4)):
+        assert call(**{written: LN[other] + off}).endswith(f"{written} overlaps {other}"), (off, error())
+
+
+@pytest.mark.parametrize("call,first,second", [(ln, "y", "stats")] + [(ln_bwd, *p) for p in itertools.combinations(("dx", "dgamma", "dbeta", "work"), 2)])
+def test_two_results_of_layer_norm(call, first, second):
+    assert "one address" in call(**{second: LN[first]}) and first in error() and second in error()
+    e = call(**{second: LN[first] + SIZE[first] - 4})
+    assert "overlaps" in e and first in e and second in e, e
+
+
+def test_layer_norm_columns_of_one_row_are_apart():
+    """two parts of rows of one pitch: y in the columns behind x's (then refused for the statistics, which are put onto x)"""
+    a = LN | dict(y=LN["x"] + 2 * WIDTH, stats=LN["x"])
+    for c, ok in ((WIDTH, True), (WIDTH - 1, False), (WIDTH + 1, True)):
+        assert lib().dp_layer_norm(a["x"], 1, ROWS, WIDTH, 2 * WIDTH + 4, a["gamma"], a["beta"], 0, 1e-6, a["x"] + 2 * c, 2 * WIDTH + 4, a["stats"], None) != 0
+        assert error().endswith("stats overlaps x" if ok else "y overlaps x"), (c, error())
+
+
+def test_layer_norm_pitches_have_a_limit():
+    far = (1 << 40) + 1
+    for xs, ys in ((far, PITCH), (PITCH, far), (1 << 62, PITCH)):
+        assert lib().dp_layer_norm(LN["x"], 1, ROWS, WIDTH, xs, None, None, 0, 1e-6, LN["y"], ys, None, None) != 0 and "pitch" in error()
+    for i in range(4):
+        p = [PITCH] * 4
+        p[i] = far
+        assert lib().dp_layer_norm_bwd(LN["dy"], p[0], LN["x"], p[1], 1, ROWS, WIDTH, None, 0, LN["stats"], LN["addend"], p[2], LN["dx"], p[3], None, None, None, 0, None) != 0
+        assert "pitch" in error()
