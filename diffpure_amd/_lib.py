@@ -66,7 +66,7 @@ SIGNATURES = {
     "dp_attention_lse_workspace": [_i, _i, _i, _i, _i, _i, _i],
     "dp_attention_lse_bwd_workspace": [_i, _i, _i, _i, _i, _i, _i],
     "dp_attention_lse_bwd": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _f, _i, _p, _p, _p, _p, _ll, _p],
-    "dp_attention_lse_bwd_f32": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _f, _i, _p, _p, _p, _p, _ll, _p],
+    "dp_attention_lse_bwd_f32": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _f, _i, _p, _p, _p, _p, _p, _ll, _p],
     "dp_layer_norm": [_p, _i, _ll, _i, _ll, _p, _p, _i, _f, _p, _ll, _p, _p],
     "dp_layer_norm_bwd_workspace": [_ll, _i, _i],
     "dp_layer_norm_bwd": [_p, _ll, _p, _ll, _i, _ll, _i, _p, _i, _p, _p, _ll, _p, _ll, _p, _p, _p, _ll, _p],

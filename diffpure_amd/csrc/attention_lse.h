@@ -363,6 +363,7 @@ struct Args {
     const int *q_lens, *kv_lens;
     int B, Tq, Tk, Hq, Hkv, D, Tqp;
     int wide;                     // backward: the gradients are fp32 whatever the operands are
+    const float* sample_scale;    // wide: [B] factors of the samples' gradients, or null
     int packed;                   // 1: the queries of all heads of a group are the columns of one block (heads share their keys)
     int splits, split_rows;       // the streamed rows are cut into `splits` ranges of split_rows
     float scale;

@@ -166,7 +166,8 @@ __device__ __forceinline__ void dq_block(const Args& p, int bid0, typename Dq<DT
     const bool out = col < kept.cols;
     const long long kr = (long long)z * kept.cols + col + (long long)split * (p.packed ? p.Hkv : p.Hq) * p.B * kept.cols;
     char* row = const_cast<char*>(p.w0.p) + b * p.w0.b + head * p.w0.h + tok * p.w0.t;
-    const float mul = some ? (AGAIN ? ldexpf(p.scale, low - T::PSHIFT) : p.scale / (float)(1 << T::PSHIFT)) : 0.f;
+    const float own = p.sample_scale ? p.sample_scale[b] * p.scale : p.scale;
+    const float mul = some ? (AGAIN ? ldexpf(own, low - T::PSHIFT) : own / (float)(1 << T::PSHIFT)) : 0.f;
     if constexpr (AGAIN) {
         join_units<DT, ND, 1>(dq, mul, smem, wave, 0, lane, [&](int u, f32x4 v) {
             const int d = Units<DT, ND>::d(u, g);
@@ -334,7 +335,7 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
             issue(cur, 0, last);
             sweep();
             const bool found = lost && fabsf(dk[0][0]) < INFINITY;
-            join_units<DT, ND, 1>(dk, col < m ? ldexpf(p.scale, low - T::PSHIFT) : 0.f, smem, wave, 0, lane, [&](int u, f32x4 v) {
+            join_units<DT, ND, 1>(dk, col < m ? ldexpf(p.sample_scale ? p.sample_scale[b] * p.scale : p.scale, low - T::PSHIFT) : 0.f, smem, wave, 0, lane, [&](int u, f32x4 v) {
                 const int d = Units<DT, ND>::d(u, g);
                 if (found && col < p.Tk && d < p.D) st4<DT>(row, d, v, p.wide);
             });
@@ -352,7 +353,7 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
     }
 
     const bool out = col < p.Tk;
-    const float pm = col < m ? 1.f / (float)(1 << T::PSHIFT) : 0.f;
+    const float pm = col < m ? (p.sample_scale ? p.sample_scale[b] : 1.f) / (float)(1 << T::PSHIFT) : 0.f;
     const long long kr = ((long long)split * p.B * p.Hkv + z) * p.Tk + col;
     auto put = [&](const typename T::Acc(&acc)[ND], float mul, const Ten& w, float* part) {
         __syncthreads();
@@ -513,7 +514,7 @@ extern "C" long long dp_attention_lse_bwd_workspace(int dtype, int B, int Tq, in
 }
 
 namespace {
-int attn_lse_bwd(const char* fn, bool wide, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides,
+int attn_lse_bwd(const char* fn, bool wide, const float* sample_scale, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides,
                  int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, void* dq, void* dk, void* dv,
                  void* work, long long work_bytes, void* stream) {
     al::Args a{};
@@ -532,9 +533,10 @@ int attn_lse_bwd(const char* fn, bool wide, const void* dout, const void* q, con
                                   dp::flat("work", work, need)},
                      read[] = {dp_attn_lse_region("q", a.q, B, Tq, Hq, row), dp_attn_lse_region("k", a.k, B, Tk, Hkv, row), dp_attn_lse_region("v", a.v, B, Tk, Hkv, row),
                                dp_attn_lse_region("out", a.o, B, Tq, Hq, row), dp_attn_lse_region("dout", a.dout, B, Tq, Hq, row), dp::flat("lse", lse, 4LL * B * Hq * Tq),
-                               dp::flat("q_lens", q_lens, 4LL * B), dp::flat("kv_lens", kv_lens, 4LL * B)};
-    if (dp::check_apart(fn, written, 4, read, 8)) return 1;
+                               dp::flat("q_lens", q_lens, 4LL * B), dp::flat("kv_lens", kv_lens, 4LL * B), dp::flat("sample_scale", sample_scale, 4LL * B)};
+    if (dp::check_apart(fn, written, 4, read, 9)) return 1;
     a.wide = wide && dtype != 0;
+    a.sample_scale = sample_scale;
     a.lse = const_cast<float*>(lse);
     a.rows = static_cast<float*>(work);
     a.lost_q = reinterpret_cast<int*>(a.rows + 2LL * B * Hq * a.Tqp);
@@ -552,12 +554,12 @@ int attn_lse_bwd(const char* fn, bool wide, const void* dout, const void* q, con
 extern "C" int dp_attention_lse_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides,
                                     int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal,
                                     void* dq, void* dk, void* dv, void* work, long long work_bytes, void* stream) {
-    return attn_lse_bwd("dp_attention_lse_bwd", false, dout, q, k, v, out, lse, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, dq, dk, dv, work,
+    return attn_lse_bwd("dp_attention_lse_bwd", false, nullptr, dout, q, k, v, out, lse, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, dq, dk, dv, work,
                         work_bytes, stream);
 }
 extern "C" int dp_attention_lse_bwd_f32(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides,
                                         int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal,
-                                        float* dq, float* dk, float* dv, void* work, long long work_bytes, void* stream) {
-    return attn_lse_bwd("dp_attention_lse_bwd_f32", true, dout, q, k, v, out, lse, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, dq, dk, dv, work,
+                                        float* dq, float* dk, float* dv, const float* sample_scale, void* work, long long work_bytes, void* stream) {
+    return attn_lse_bwd("dp_attention_lse_bwd_f32", true, sample_scale, dout, q, k, v, out, lse, strides, dtype, B, Tq, Tk, Hq, Hkv, D, q_lens, kv_lens, scale, causal, dq, dk, dv, work,
                         work_bytes, stream);
 }

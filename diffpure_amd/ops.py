@@ -1117,10 +1117,11 @@ def attention_lse(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
     return out, lse
 
 
-def attention_lse_bwd(dout, q, k, v, out, lse, scale=None, causal=False, q_lens=None, kv_lens=None, grads=None):
+def attention_lse_bwd(dout, q, k, v, out, lse, scale=None, causal=False, q_lens=None, kv_lens=None, grads=None, sample_scale=None):
     """Gradients (dq, dk, dv) of attention_lse's `out` for the cotangent dout, given its results and the arguments of the forward call.  No [Tq, Tk] tensor
     and no atomics; a key head's gradient is the sum over the query heads that share it.  grads=(dq, dk, dv): written into these tensors (of
-    q's type, or all three fp32; views of one dqkv tensor, say, that lies apart from every input) instead of new contiguous ones."""
+    q's type, or all three fp32; views of one dqkv tensor, say, that lies apart from every input) instead of new contiguous ones.  sample_scale: with fp32 grads, fp32 [B] - each
+    sample's gradients are multiplied by it."""
     st, args = _attn_lse_args("attention_lse_bwd", q, k, v, scale, q_lens, kv_lens)
     b, tq, hq, d = q.shape
     st += _heads(out, "attention_lse_bwd.out", q, q.shape) + _heads(dout, "attention_lse_bwd.dout", q, q.shape)
@@ -1133,11 +1134,14 @@ def attention_lse_bwd(dout, q, k, v, out, lse, scale=None, causal=False, q_lens=
         f32 = isinstance(dq, torch.Tensor) and dq.dtype == torch.float32
         for t, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
             st += _heads(t, f"attention_lse_bwd.{name}", dq if f32 and dq.device == q.device else q, like.shape)
+        if sample_scale is not None and (not f32 or not isinstance(sample_scale, torch.Tensor) or sample_scale.device != q.device or sample_scale.dtype != torch.float32 or
+                                         sample_scale.dim() != 1 or sample_scale.shape[0] != b or not sample_scale.is_contiguous()):
+            raise _lib.DiffpureHipError(f"attention_lse_bwd.sample_scale: expected contiguous float32 [{b}] on {q.device}, and float32 grads")
         st = (ctypes.c_longlong * 24)(*st)
         nbytes = _lib.load().dp_attention_lse_bwd_workspace(*args[:7])
         work = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32)
         _lib.call("dp_attention_lse_bwd_f32" if f32 else "dp_attention_lse_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), ctypes.addressof(st), *args, int(bool(causal)),
-                  _ptr(dq), _ptr(dk), _ptr(dv), _ptr(work), nbytes, _stream())
+                  _ptr(dq), _ptr(dk), _ptr(dv), *([_ptr(sample_scale)] if f32 else []), _ptr(work), nbytes, _stream())
     return dq, dk, dv
 
 
@@ -1150,8 +1154,8 @@ def attention_recompute_wanted(d):
 
 def attention_recompute_bwd(qkv, dout, n_heads, layout):
     """attention_bwd without the probabilities: d qkv [B, T, 3C] (fp32) for dout [B, T, C] fp32, q, k and v read in place from qkv (fp32 or the taped
-    fp16 tensor, whose type the products' operands then have).  With fp16 operands each sample's dout is brought to a largest element of 4 to 8 by a power of
-    two on its way into them, and d qkv back: results follow dout's size exactly, however small or large."""
+    fp16 tensor, whose type the products' operands then have).  With fp16 operands each sample's dout is brought to a largest element of 1 to 2 by a power of
+    two on its way into them, and d qkv back: results follow dout's size exactly, however small or large (from 2^-100 on)."""
     if not isinstance(qkv, torch.Tensor) or not qkv.is_cuda or qkv.dim() != 3 or qkv.dtype not in (torch.float32, torch.float16) or not qkv.is_contiguous():
         raise _lib.DiffpureHipError("attention_recompute_bwd.qkv: expected a contiguous float32 or float16 GPU tensor [B, T, 3C]")
     b, t, c3 = qkv.shape
@@ -1168,11 +1172,12 @@ def attention_recompute_bwd(qkv, dout, n_heads, layout):
         attention_lse_bwd(dout.view(b, t, n_heads, d), q, k, v, out, lse, grads=heads(dqkv))
         return dqkv
     # (two steps: a reduction over a whole sample in one would need a cleared counter, which a captured graph must not)
-    e = 3.0 - torch.frexp(torch.linalg.vector_norm(dout, ord=math.inf, dim=2).amax(dim=1)).exponent.clamp(-100, 100).float().view(b, 1, 1)
+    top = torch.linalg.vector_norm(dout, ord=math.inf, dim=2).amax(dim=1)
+    power = (top.view(torch.int32) & 0x7F800000).view(torch.float32).clamp_min_(2.0 ** -100)         # 2^floor(log2 top); not finite where dout is not
     scaled = torch.empty(dout.shape, device=dout.device, dtype=qkv.dtype)
-    torch.mul(dout, torch.exp2(e), out=scaled)
-    attention_lse_bwd(scaled.view(b, t, n_heads, d), q, k, v, out, lse, grads=heads(dqkv))
-    return dqkv.mul_(torch.exp2(-e))
+    torch.div(dout, power.view(b, 1, 1), out=scaled)
+    attention_lse_bwd(scaled.view(b, t, n_heads, d), q, k, v, out, lse, grads=heads(dqkv), sample_scale=power)
+    return dqkv
 
 
 # ---------------------------------------------------------------------------------------------

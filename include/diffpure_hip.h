@@ -435,10 +435,11 @@ long long dp_attention_lse_bwd_workspace(int dtype, int B, int Tq, int Tk, int H
 int dp_attention_lse_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides, int dtype,
                          int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, void* dq, void* dk,
                          void* dv, void* work, long long work_bytes, void* stream);
-/* The same with dq, dk and dv in fp32 whatever dtype is (their strides in fp32 elements): sums that no 16-bit range cuts off, for callers that scale dout. */
+/* The same with dq, dk and dv in fp32 whatever dtype is (their strides in fp32 elements): sums that no 16-bit range cuts off, for callers that scale dout on its way into
+ * a 16-bit type.  sample_scale: device fp32 [B] or NULL - what each sample's gradients are multiplied by as they are written. */
 int dp_attention_lse_bwd_f32(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const long long* strides, int dtype,
                              int B, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_lens, const int* kv_lens, float scale, int causal, float* dq,
-                             float* dk, float* dv, void* work, long long work_bytes, void* stream);
+                             float* dk, float* dv, const float* sample_scale, void* work, long long work_bytes, void* stream);
 
 /* ---- layer norm over the last axis, and its backward pass with the weights' gradients ---------------------------------
  *   y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(var + eps) (biased variance); stats[row] = (mean, rstd) fp32, or NULL.

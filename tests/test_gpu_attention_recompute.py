@@ -162,3 +162,33 @@ def test_refusals_of_fp32_gradients():
     wide = torch.empty(1, 8, 2, 17, device=DEV)
     with pytest.raises(DiffpureHipError, match="strides"):
         ops.attention_lse_bwd(dout, q, k, v, out, lse, grads=(wide[..., :16], f[1], f[2]))
+
+
+@pytest.mark.gpu
+def test_sample_scale_is_a_factor_of_the_gradients():
+    """powers of two: the bits of the unscaled call times the factor, in every form of a launch and for fp32 operands too; what else it is is refused"""
+    from diffpure_amd import ops
+    from diffpure_amd._lib import DiffpureHipError
+    from test_gpu_attention_lse import SHAPES, lens_of, make
+    for dtype in (torch.float16, torch.float32):
+        for n, (b, tq, tk, hq, hkv, d, causal, ql, kl, layout) in enumerate(SHAPES):
+            q, k, v, dout = make(dtype, b, tq, tk, hq, hkv, d, layout, seed=n)
+            ql, kl = (None if x is None else lens_of(*x) for x in (ql, kl))
+            out, lse = ops.attention_lse(q, k, v, None, causal, ql, kl)
+            factor = torch.tensor([2.0 ** (11 * i - 20) for i in range(b)], device=DEV)        # (made on the host: the GPU's pow(2, 24) is 16777215)
+            grads = lambda: tuple(torch.empty(t.shape, device=DEV) for t in (q, k, v))
+            want = ops.attention_lse_bwd(dout, q, k, v, out, lse, None, causal, ql, kl, grads=grads())
+            got = ops.attention_lse_bwd(dout, q, k, v, out, lse, None, causal, ql, kl, grads=grads(), sample_scale=factor)
+            for a, w in zip(got, want):
+                assert torch.equal(a, w * factor.view(b, 1, 1, 1)), (dtype, n)
+    q = torch.randn(2, 8, 2, 16, device=DEV).half()
+    k, v, dout = q.clone(), q.clone(), q.clone()
+    out, lse = ops.attention_lse(q, k, v)
+    f = [torch.empty(q.shape, device=DEV) for _ in range(3)]
+    for bad in (torch.ones(3, device=DEV), torch.ones(2, device=DEV, dtype=torch.float64), torch.ones(2), torch.ones(2, 1, device=DEV), torch.ones(4, device=DEV)[::2], 2.0):
+        with pytest.raises(DiffpureHipError, match="sample_scale"):
+            ops.attention_lse_bwd(dout, q, k, v, out, lse, grads=f, sample_scale=bad)
+    with pytest.raises(DiffpureHipError, match="sample_scale"):
+        ops.attention_lse_bwd(dout, q, k, v, out, lse, sample_scale=torch.ones(2, device=DEV))
+    with pytest.raises(DiffpureHipError, match="sample_scale"):                       # on what the call writes
+        ops.attention_lse_bwd(dout, q, k, v, out, lse, grads=f, sample_scale=f[1].view(-1)[:2])

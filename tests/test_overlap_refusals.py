@@ -31,7 +31,7 @@ def bwd(f32=False, strides=None, **at):
     fn = lib().dp_attention_lse_bwd_f32 if f32 else lib().dp_attention_lse_bwd
     need = lib().dp_attention_lse_bwd_workspace(1, B, T, T, H, H, D)
     assert fn(a["dout"], a["q"], a["k"], a["v"], a["out"], a["lse"], C.addressof(arr), 1, B, T, T, H, H, D, a["q_lens"], a["kv_lens"], 0.25, 0, a["dq"], a["dk"],
-              a["dv"], a["work"], need, None) != 0
+              a["dv"], *([None] if f32 else []), a["work"], need, None) != 0
     return error()
 
 
