@@ -36,7 +36,8 @@ __device__ __forceinline__ void settle() {
 }
 
 // at least `n` waves per SIMD: with 2 the registers of a wave end at 256 and the matrix instructions take their accumulators from the ordinary
-// ones (with more, they move through the accumulation registers and every score tile is copied)
+// ones (with one wave they move through the accumulation registers and score tiles are copied).  Forms whose waves share columns miss that from 96 channels on: their
+// stages fill 98 KB of LDS and more, one workgroup to a CU, and the compiler then spreads over the accumulation registers too (28 to 123 of them).
 #define AL_WAVES(n) __attribute__((amdgpu_waves_per_eu(n)))
 
 constexpr float LOG2E = 1.44269504088896341f;

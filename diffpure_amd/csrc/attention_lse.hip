@@ -2,11 +2,14 @@
 // dimensions up to 256 and types: what a backward pass that recomputes the probabilities (attention_lse_bwd.hip) starts from.
 //
 // One pass over the keys with a running maximum and sum per query; the scores of a tile never leave the registers.  Measured on MI355X:
-//   64 x 1024 tokens, 8 heads of 64, fp16    190 us, 725 TFLOP/s: bound by the VALU - per 32 x 32 tile 256 cycles of exp2 (16 per wave instruction) and 280 of
-//                                            everything else against 256 of matrix instructions, four waves per SIMD
-//   64 x 197 tokens, 12 heads of 64, bf16    22.6 us
-//   4 x 1 query, 50 001 keys, 16 / 4 heads of 128, bf16    91 us = 4.5 TB/s: the heads of a group packed into one tile, four waves on different rows,
-//                                            16 ranges of keys joined by a second launch (7 us)
+//   64 x 1024 tokens, 8 heads of 64, fp16    192 us (whole call), 715 TFLOP/s: by the counters vector instructions keep a SIMD busy for 75 % of the launch and matrix
+//                                            instructions for 36 %, so the two hardly overlap, though 119 registers leave four waves per SIMD; 108 vector
+//                                            instructions per 32 x 32 tile, of which 16 exponentials (16 cycles each)
+//   64 x 197 tokens, 12 heads of 64, bf16    24 us: 1.48 times the work (128-column blocks, 32-key tiles), short workgroups
+//   4 x 1 query, 50 001 keys, 16 / 4 heads of 128, bf16    90.5 us = 4.5 TB/s: the heads of a group packed into one tile, four waves on different rows,
+//                                            16 ranges of keys joined by a second launch (5 us)
+//   32 x 1024 tokens, 8 heads of 64, fp32    604 us = 114 TFLOP/s of the 154 that a large fp32 product reaches
+// Above 128 channels the fp32 form spills 27 registers (128 x 256 tokens x 1 head of 256: 92 us, its operations 56).
 #include "attention_lse.h"
 
 namespace {

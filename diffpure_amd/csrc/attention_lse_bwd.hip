@@ -5,12 +5,12 @@
 // Two kernels, no atomics (results do not depend on the order of workgroups): dQ keeps queries and streams keys (and writes delta and the
 // log2-domain log-sum-exp, +inf where a row has no gradient, for the other), dK / dV keeps keys and streams the queries of every head of its group.
 //
-// Measured on MI355X:
-//   32 x 1024 tokens, 8 heads of 64, fp16    280 us (dQ 137, dK / dV 182 by the profiler's clock, 0.75 PFLOP/s each): bound by the VALU, which forms the
-//                                            exponential in both (16 cycles per wave instruction)
-//   8191 tokens causal, 16 / 4 heads of 128, bf16    1107 us (dQ 380, dK and dV 740: 1.0 and 0.93 PFLOP/s): bound by the matrix instructions of 8 products
-//   128 x 256 tokens, one head of 256, fp16    75 us, of which 30 are kept operands and results
-//   1 x 256 tokens, 16 heads of 64, fp32    20 us: two launches of four stages, latency
+// Measured on MI355X (whole calls, warm; kernels by the profiler's clock, mean and least of 100):
+//   32 x 1024 tokens, 8 heads of 64, fp16    290 us; dQ 132 and 122: matrix instructions keep a SIMD busy for 39 % of it, vector instructions for 47 %; dK and dV 166 and
+//                                            153: 33 % and 34 %, the rest is waiting (a barrier per tile, three waves per SIMD)
+//   8191 tokens causal, 16 / 4 heads of 128, bf16    1120 us; dQ 391 and 380, dK and dV 743 and 713, joining two ranges 14: bound by the matrix instructions of 8 products
+//   128 x 256 tokens, one head of 256, fp16    79 us; dQ 31, dK and dV 49, of which 30 are kept operands and results
+//   1 x 256 tokens, 16 heads of 64, fp32    20 us; 11 each: two launches of four stages, latency
 //
 // fp16: the probabilities are formed as 2^6 P (an addend of the exponent) and taken out of the sums again at the end.  dS is rounded to fp16 as
 // operand of its product, and P (dP - delta) of a long row is easily 1e-3 of dout: without the factor it meets fp16's subnormals (below 6e-5) six
