@@ -15,9 +15,10 @@
 // fp16: the probabilities are formed as 2^6 P (an addend of the exponent) and taken out of the sums again at the end.  dS is rounded to fp16 as
 // operand of its product, and P (dP - delta) of a long row is easily 1e-3 of dout: without the factor it meets fp16's subnormals (below 6e-5) six
 // bits earlier.  Large cotangents (a scaled loss) bring 2^6 dS, or dS itself, beyond 65504.  Such an element is infinite, and so, or NaN, is every sum that it
-// enters: a wave that finds one says so, and a last launch (attn_lse_again: 4 us where there is none) forms those columns anew, with 2^-6, 2^-18 and 2^-30 dS
-// (|dS| < 2^39) until they are finite - or lost because the input is.  In tiles of the first two launches a test for it costs more (dQ of 32 x 1024 tokens x 8 heads:
-// 122 us, 128 with a running maximum of |dS|, 140 with a second loop in the same kernel, whose registers the first then lacks).
+// enters: a wave that finds one says so, and a last launch (attn_lse_again) forms those columns anew, with 2^-6, 2^-18 and 2^-30 dS (|dS| < 2^39) until they are
+// finite - or lost because the input is.  It costs 4 us where nothing was lost; with every column lost 32 x 1024 x 8 heads of 64 take 725 us instead of 290, with all of
+// dout NaN 1250.  In tiles of the first two launches a test for it costs more (dQ of the same: 122 us, 128 with a running maximum of |dS|, 140 with a second loop in
+// the same kernel, whose registers the first then lacks).
 #include "attention_lse.h"
 
 namespace {
@@ -383,27 +384,27 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
     } else dkv_block<DT, DP, RS, 3, false>(p, bid, sh);
 }
 
-// fp16: what the launches before lost, first the queries' blocks, then the keys'.  Nothing is shared with another workgroup, and nothing cut into ranges.  One workgroup
-// per CU takes `per` blocks, and leaves if nothing was lost in the key heads that they belong to.
+// fp16: what the launches before lost.  Nothing is shared with another workgroup, and nothing cut into ranges.  Two workgroups per CU take q_per blocks of queries and
+// k_per of keys each, and leave if nothing was lost in the key heads that these belong to.
 template <int DT, int DP>
-__global__ __launch_bounds__(256) AL_WAVES(DP > 64 ? 1 : 2) void attn_lse_again_kernel(Args p, int q_blocks, int blocks, int per) {
+__global__ __launch_bounds__(256) AL_WAVES(2) void attn_lse_again_kernel(Args p, int q_blocks, int q_per, int k_blocks, int k_per) {
     __shared__ __attribute__((aligned(1024))) union {
         typename Dq<DT, DP, 1>::Shared q;
         typename Dkv<DT, DP, 1>::Shared k;
     } sh;
     constexpr int COLS = 4 * Tr<DT>::TILE;
-    const int begin = blockIdx.x * per, end = min(begin + per, blocks), q_end = min(end, q_blocks), k_begin = max(begin, q_blocks);
+    const int q0 = min((int)blockIdx.x * q_per, q_blocks), q1 = min(q0 + q_per, q_blocks), k0 = min((int)blockIdx.x * k_per, k_blocks), k1 = min(k0 + k_per, k_blocks);
     const int qn = (p.Tq + COLS - 1) / COLS * (p.Hq / p.Hkv), kn = (p.Tk + COLS - 1) / COLS;       // blocks of a key head
     int any = 0;
     auto look = [&](const int* lost, int n, int z0, int z1) {
         for (long long i = (long long)z0 * n + threadIdx.x; i < (z1 + 1LL) * n; i += 256) any |= lost[i];
     };
-    if (begin < q_end) look(p.lost_q, p.lost_qn, begin / qn, (q_end - 1) / qn);
-    if (k_begin < end) look(p.lost_k, p.lost_kn, (k_begin - q_blocks) / kn, (end - 1 - q_blocks) / kn);
+    if (q0 < q1) look(p.lost_q, p.lost_qn, q0 / qn, (q1 - 1) / qn);
+    if (k0 < k1) look(p.lost_k, p.lost_kn, k0 / kn, (k1 - 1) / kn);
     if (!__syncthreads_or(any)) return;
-    for (int i = begin; i < q_end; ++i) dq_block<DT, DP, 1, true>(p, i, sh.q);
+    for (int i = q0; i < q1; ++i) dq_block<DT, DP, 1, true>(p, i, sh.q);
     __syncthreads();
-    for (int i = k_begin; i < end; ++i) dkv_block<DT, DP, 1, 1, true>(p, i - q_blocks, sh.k);
+    for (int i = k0; i < k1; ++i) dkv_block<DT, DP, 1, 1, true>(p, i, sh.k);
 }
 
 // sums of the ranges of a split launch, in their order: part [split][rows][D] -> rows of a [B, T, H, D] tensor.  Packed as the kept queries are, or plain
@@ -486,8 +487,8 @@ void launch_bwd(const Args& a, const Ten& dq, const Ten& dk, const Ten& dv, hipS
         x.stripes = 1;
         x.lost_qn = (int)(q_waves(pq) / ((long long)a.B * a.Hkv));
         x.lost_kn = (int)(k_waves(pk, DP) / ((long long)a.B * a.Hkv));
-        const int per = (qb + kb + 255) / 256;
-        hipLaunchKernelGGL((attn_lse_again_kernel<DT, DP>), dim3((unsigned)((qb + kb + per - 1) / per)), wg, 0, s, x, qb, qb + kb, per);
+        const int most = qb > kb ? qb : kb, wgs = most < 512 ? most : 512;
+        hipLaunchKernelGGL((attn_lse_again_kernel<DT, DP>), dim3((unsigned)wgs), wg, 0, s, x, qb, (qb + wgs - 1) / wgs, kb, (kb + wgs - 1) / wgs);
     }
 }
 template <int DTYPE>
