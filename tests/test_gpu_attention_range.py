@@ -91,3 +91,46 @@ def test_rows_that_are_not_finite_do_not_choose_the_factor():
     rest[9] = False
     close(dq[:, rest.cuda(), 0], res[0][:, rest, 0], tol[0][:, rest, 0], "dq")
     close(dq[:, :, 1], res[0][:, :, 1], tol[0][:, :, 1], "dq of the other head")
+
+
+@pytest.mark.parametrize("form", ["own", "causal", "wide", "few_keys"])
+def test_lost_and_ordinary_calls_in_turn(form):
+    """eager twice, on another stream, and replayed from two graphs: ordinary cotangents, ones whose dS overflow, and NaN follow one another in the same buffers; every
+    result has the bits of the eager call"""
+    from diffpure_amd import ops
+    q, k, v, dout, causal = inputs(form, (1.0, 1.0))
+    q, k, v, dout = (t.cuda() for t in (q, k, v, dout))
+    b, tq, tk = q.shape[0], q.shape[1], k.shape[1]
+    ql, kl = lens_of(*[tq - 3 * i for i in range(b)]), lens_of(*[tk - 2 * i for i in range(b)])
+    out, lse = ops.attention_lse(q, k, v, None, causal, ql, kl)
+    base = dout.clone()
+
+    def step():
+        return ops.attention_lse_bwd(dout, q, k, v, out, lse, None, causal, ql, kl)
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step()
+        graphs.append((g, res))
+    side = torch.cuda.Stream()
+    for size in (1.0, 2e4, 1.0, math.nan, 2e4, 1e-3, 2e4):
+        dout.copy_(base)
+        if size == size:
+            dout.copy_((base.float() * size).half())
+        else:
+            dout[0, 0, 0] = size
+        for g, _ in graphs:
+            g.replay()
+        want = step()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        if size == size:
+            assert all(torch.isfinite(t).all() for t in want), size
+        for res in [other] + [r for _, r in graphs]:
+            assert all(torch.equal(a.view(torch.int16), c.view(torch.int16)) for a, c in zip(res, want)), size

@@ -157,6 +157,14 @@ def test_usual_views_pass():
                     ([T * (d3 + 8), d3 + 8, 3 * D], D), ([T * (d3 + 8) + 16, d3 + 8, 3 * D], D), ([D, B * H * 3 * D, 3 * B * D], B * D)):
         e = bwd(strides={"dq": s, "dk": s, "dv": s}, dk=AT["dq"] + 2 * step, dv=AT["dq"])
         assert e.endswith("dq and dv begin at one address"), e
+    # query heads and the key heads that they share in one projection's gradient: [dq of 4 heads | dk of 2 | dv of 2], and dv one head short of its place
+    w = 8 * D
+    for at, e in ((AT["dq"] + 2 * 6 * D, None), (AT["dq"] + 2 * 5 * D, "dk overlaps dv")):
+        st = (C.c_longlong * 24)(*([T * 4 * D, 4 * D, D] + [T * 2 * D, 2 * D, D] * 2 + [T * 4 * D, 4 * D, D] * 2 + [T * w, w, D] * 3))
+        dout = AT["dout"] if e else AT["work"]             # (on the workspace: refused for that if nothing before it is)
+        assert lib().dp_attention_lse_bwd(dout, AT["q"], AT["k"], AT["v"], AT["out"], AT["lse"], C.addressof(st), 1, B, T, T, 4, 2, D, None, None, 0.25, 0, AT["dq"],
+                                          AT["dq"] + 2 * 4 * D, at, AT["work"], MB, None) != 0
+        assert error().endswith(e or "work overlaps dout"), error()
     # one sample, one token, heads apart
     st = (C.c_longlong * 24)(*([H * D, H * D, D] * 5 + [0, 0, 3 * D] * 3))
     assert lib().dp_attention_lse_bwd(AT["dout"], AT["q"], AT["k"], AT["v"], AT["out"], AT["lse"], C.addressof(st), 1, 1, 1, 1, H, H, D, None, None, 0.25, 0, AT["dq"],
