@@ -28,12 +28,24 @@ template <int DT, int DP, int RS> struct Dq {
     using St = Stream<DP * Tr<DT>::ES, Tr<DT>::ES, RS * Tr<DT>::ROWS, 4>;
     struct Shared { char stage[2 * St::STAGE]; };
 };
-// an fp16 (or, wide, fp32) element of a written tensor that is infinite or NaN
-__device__ __forceinline__ bool not_finite(const char* x, int wide) {
-    return wide ? (*reinterpret_cast<const unsigned*>(x) & 0x7f800000) == 0x7f800000 : (*reinterpret_cast<const unsigned short*>(x) & 0x7c00) == 0x7c00;
+// A column that an infinite dS entered: ALL of its channels are infinite or NaN (the operand that it multiplies is something in each).  One channel alone is an operand's:
+// a key of an infinite channel and weight 0, say, whose other channels stand.  Of the sums, and of an fp16 (or, wide, fp32) row of D elements:
+template <int DT, int ND> __device__ __forceinline__ bool lost_sums(const typename Tr<DT>::Acc (&acc)[ND]) {
+    bool all = true;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int r = 0; r < Tr<DT>::NR; ++r) all = all && !(fabsf(acc[dt][r]) < INFINITY);
+    return col_reduce<Tr<DT>::TILE>(all ? 1.f : 0.f, [](float a, float b) { return fminf(a, b); }) > 0.f;
+}
+template <int DT> __device__ __forceinline__ bool lost_row(const char* x, int D, int g, int wide) {
+    bool all = true;
+    for (int d = g; d < D; d += Tr<DT>::G)
+        all = all && (wide ? (reinterpret_cast<const unsigned*>(x)[d] & 0x7f800000) == 0x7f800000 : (reinterpret_cast<const unsigned short*>(x)[d] & 0x7c00) == 0x7c00);
+    return col_reduce<Tr<DT>::TILE>(all ? 1.f : 0.f, [](float a, float b) { return fminf(a, b); }) > 0.f;
 }
 
-// dQ.  Workgroups, stages and RS as in the forward kernel.  AGAIN: the queries among the workgroup's whose dq (all of a query's channels, or none) is not finite.
+// dQ.  Workgroups, stages and RS as in the forward kernel.  AGAIN: the queries among the workgroup's that were lost.
 template <int DT, int DP, int RS, bool AGAIN>
 __device__ __forceinline__ void dq_block(const Args& p, int bid0, typename Dq<DT, DP, RS>::Shared& sh) {
     using T = Tr<DT>;
@@ -59,7 +71,7 @@ __device__ __forceinline__ void dq_block(const Args& p, int bid0, typename Dq<DT
     kept.col(p, col < kept.cols ? col : kept.cols - 1, head, tok);
     bool lost = false;
     if constexpr (AGAIN) {
-        lost = not_finite(p.w0.p + b * p.w0.b + head * p.w0.h + tok * p.w0.t, p.wide);
+        lost = lost_row<DT>(p.w0.p + b * p.w0.b + head * p.w0.h + tok * p.w0.t, p.D, g, p.wide);
         if (!__syncthreads_or(lost)) return;
     }
     const int krow = tok < n ? tok : (n > 0 ? n - 1 : 0);
@@ -153,8 +165,9 @@ __device__ __forceinline__ void dq_block(const Args& p, int bid0, typename Dq<DT
             for (int dt = 0; dt < ND; ++dt) dq[dt] = typename T::Acc{};
             if (begin < end) st.issue(smem + cur * St::STAGE, begin, m, 0, 0);
             sweep();
-            still = !(fabsf(dq[0][0]) < INFINITY);
+            still = lost_sums<DT, ND>(dq);
         } while (__syncthreads_or(still && low < 36));
+        lost = lost && !still;                    // (what stays lost is the input's: it stands as it is)
     } else {
         sweep();
         if constexpr (T::PSHIFT > 0) {
@@ -197,7 +210,7 @@ __global__ __launch_bounds__(256) AL_WAVES(DT == 0 && DP > 128 ? 1 : DT && DP ==
 }
 
 // dK and dV: keys are kept, the queries of every head of the group stream by, one head after the other.  WHAT: 1 dK, 2 dV, 3 both.  AGAIN: the dK among the workgroup's
-// that are not finite; they take their exponents' addends lowered, the same for all, and a key's dK is that of the first pass in which it is finite.
+// that were lost; they take their exponents' addends lowered, the same for all, and a key's dK is that of the first pass in which it is finite.
 template <int DT, int DP, int RS> struct Dkv {
     static constexpr int NW = 4, BM = RS * Tr<DT>::ROWS, RB = DP * Tr<DT>::ES, STATS = 2 * BM < 64 ? 64 : 2 * BM;
     using St = Stream<RB, Tr<DT>::ES, BM, NW>;
@@ -229,7 +242,7 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
 
     bool lost = false;
     if constexpr (AGAIN) {
-        lost = not_finite(p.w1.p + b * p.w1.b + hk * p.w1.h + (col < p.Tk ? col : p.Tk - 1) * p.w1.t, p.wide);
+        lost = lost_row<DT>(p.w1.p + b * p.w1.b + hk * p.w1.h + (col < p.Tk ? col : p.Tk - 1) * p.w1.t, p.D, g, p.wide);
         if (!__syncthreads_or(lost)) return;
     }
     typename T::Frag kf[KS], vf[DK ? KS : 1];
@@ -335,7 +348,7 @@ __device__ __forceinline__ void dkv_block(const Args& p, int bid0, typename Dkv<
             for (int dt = 0; dt < ND; ++dt) dk[dt] = typename T::Acc{};
             issue(cur, 0, last);
             sweep();
-            const bool found = lost && fabsf(dk[0][0]) < INFINITY;
+            const bool found = lost && !lost_sums<DT, ND>(dk);
             join_units<DT, ND, 1>(dk, col < m ? ldexpf(p.sample_scale ? p.sample_scale[b] * p.scale : p.scale, low - T::PSHIFT) : 0.f, smem, wave, 0, lane, [&](int u, f32x4 v) {
                 const int d = Units<DT, ND>::d(u, g);
                 if (found && col < p.Tk && d < p.D) st4<DT>(row, d, v, p.wide);

@@ -420,7 +420,8 @@ int dp_resize_affine_bwd(const float* dy, int B, int C, int Ho, int Wo, int out_
  *   causal != 0: row i of a sample sees keys 0 .. i + (keys - rows) of it (the last row sees every key).  Inside the lengths values must be finite for the mask to
  *     hide them.  A row that sees no key (by the lengths and causal alone) has out 0, lse -inf, and contributes no gradient.  A row that sees a score of NaN or
  *     +inf (finite inputs may overflow to it) has NaN in out and lse; one whose scores are all -inf has out NaN, lse -inf.  The backward pass carries it on: dq of a row whose lse is NaN,
- *     and dk, dv of the keys it sees, are NaN.
+ *     and dk, dv of the keys it sees, are NaN.  A key with an infinite channel and a score of -inf has weight 0, and dq NaN in that channel alone - where D is 32, 64, 96,
+ *     128 or 256, or the channel is not among the last 8 (fp32: 4); else the score is NaN.
  *   scale: finite, not 0.
  *   work: dp_attention_lse_workspace / dp_attention_lse_bwd_workspace bytes, 16-byte aligned, free again when the call's work on `stream` is done (the
  *     forward pass needs none - 0 - where the queries fill the chip).  Whatever a call writes (gradients, out, lse, work)

@@ -134,3 +134,33 @@ def test_lost_and_ordinary_calls_in_turn(form):
             assert all(torch.isfinite(t).all() for t in want), size
         for res in [other] + [r for _, r in graphs]:
             assert all(torch.equal(a.view(torch.int16), c.view(torch.int16)) for a, c in zip(res, want)), size
+
+
+@pytest.mark.parametrize("form", ["own", "shared", "causal", "wide", "odd", "few_queries"])
+@pytest.mark.parametrize("channel", [0, 4, -1])
+@pytest.mark.parametrize("size", [1.0, 2e4])
+def test_a_key_that_is_infinite_in_one_channel(form, channel, size):
+    """its score is -inf: weight 0, and 0 * inf in that channel of dq alone.  The other channels are what they are without the key, whether dS overflows on the way or not; dk and
+    dv of every key too (0 of this one)"""
+    from diffpure_amd import ops
+    q, k, v, dout, causal = inputs(form, (size, 1.0))
+    if channel == -1 and q.shape[3] not in (64, 96, 128, 256):
+        pytest.skip("the last channels also fill a narrower head up to the kernel's width: its scores are NaN")
+    channel %= q.shape[3]
+    q[..., channel], k[..., channel] = 1.0, 0.0
+    at = k.shape[1] // 2
+    z = k.clone()
+    z[:, at, :, channel] = -100 * q.shape[3] ** 0.5                  # the definition's: exp(-100) is nothing beside the others
+    ref = Ref(q, z, v, None, causal, None, None)
+    res, tol = expected(ref, dout)
+    k[:, at, :, channel] = -math.inf
+    q, k, v, dout = (t.cuda() for t in (q, k, v, dout))
+    out, lse = ops.attention_lse(q, k, v, None, causal)
+    close(out, ref.back(ref.o), ref.out_tol(), "out")
+    dq, dk, dv = ops.attention_lse_bwd(dout, q, k, v, out, lse, None, causal)
+    rest = [c for c in range(q.shape[3]) if c != channel]
+    close(dq[..., rest], res[0][..., rest], tol[0][..., rest], "dq")
+    seen = (ref.keep[0, 0, :, at]).cuda()
+    assert torch.isnan(dq[:, seen][..., channel]).all()
+    close(dk, res[1], tol[1], "dk")
+    close(dv, res[2], tol[2], "dv")
