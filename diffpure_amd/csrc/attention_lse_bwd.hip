@@ -16,8 +16,8 @@
 // operand of its product, and P (dP - delta) of a long row is easily 1e-3 of dout: without the factor it meets fp16's subnormals (below 6e-5) six
 // bits earlier.  Large cotangents (a scaled loss) bring 2^6 dS, or dS itself, beyond 65504.  Such an element is infinite, and so, or NaN, is every sum that it
 // enters: a wave that finds one says so, and a last launch (attn_lse_again) forms those columns anew, with 2^-6, 2^-18 and 2^-30 dS (|dS| < 2^39) until they are
-// finite - or lost because the input is.  It costs 4 us where nothing was lost; with every column lost 32 x 1024 x 8 heads of 64 take 725 us instead of 290, with all of
-// dout NaN 1250.  In tiles of the first two launches a test for it costs more (dQ of the same: 122 us, 128 with a running maximum of |dS|, 140 with a second loop in
+// finite - or lost because the input is.  It costs 4 us where nothing was lost; with every column lost 32 x 1024 x 8 heads of 64 take 770 us instead of 290, with all of
+// dout NaN 1270.  In tiles of the first two launches a test for it costs more (dQ of the same: 122 us, 128 with a running maximum of |dS|, 140 with a second loop in
 // the same kernel, whose registers the first then lacks).
 #include "attention_lse.h"
 

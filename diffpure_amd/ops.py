@@ -1104,7 +1104,7 @@ def attention_lse(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
     lse [B, Hq, Tq] fp32.  fp32 / fp16 / bf16, any strides that are multiples of 16 bytes (views of one qkv tensor in either head order), any token
     counts from 1, D a multiple of 8 up to 256, Hq a multiple of Hkv (query heads h * Hq / Hkv ... share key head h); scale None = 1 / sqrt(D).
     q_lens / kv_lens: int32 [B], valid tokens per sample; causal: the last valid row sees every valid key, each row before it one fewer.
-    Rows that see nothing give 0 and -inf.  The statistics are what attention_lse_bwd recomputes the probabilities from (csrc/attention_lse.hip)."""
+    Rows that see nothing give 0 and -inf; a score of NaN or +inf makes its row NaN in both.  The statistics are what attention_lse_bwd recomputes the probabilities from (csrc/attention_lse.hip)."""
     st, args = _attn_lse_args("attention_lse", q, k, v, scale, q_lens, kv_lens)
     b, tq, hq, d = q.shape
     with torch.cuda.device(q.device):
